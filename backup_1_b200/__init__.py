@@ -19,6 +19,14 @@ from .lib import (  # noqa: F401
     ACT_RELU,
     ACT_SIGMOID,
     ACT_TANH,
+    BF16,
+    F16,
+    F32,
+    FP8_E4M3,
+    FP8_E5M2,
+    Fp8Matrix,
+    SCALE_AMAX,
+    SCALE_POW2,
     CONV_EXPLICIT,
     CONV_IMPLICIT,
     CONV_NO_COMPENSATE,

@@ -1,0 +1,177 @@
+/* Shared by the 8-bit linear layer's kernels: element types, 8-element vectors, fp8 codes and scales, argument checks. */
+#ifndef DECXB_FP8_CUH_
+#define DECXB_FP8_CUH_
+
+#include "common.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+namespace fp8 {
+
+/* ------------------------------------------------------------------ elements --------- */
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ T from_f32(float x);
+template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+/* Eight consecutive elements of a row as floats.  `n` of them exist (the others read as 0); `vec`: the
+ * address is 16-byte aligned, so a whole vector moves in 128-bit accesses. */
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int n, bool vec, float* v)
+{
+    if (n >= 8 && vec) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 a = *reinterpret_cast<const float4*>(p), b = *(reinterpret_cast<const float4*>(p) + 1);
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
+            const uint4 u = *reinterpret_cast<const uint4*>(p);
+            const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = to_f32(e[j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = j < n ? to_f32(p[j]) : 0.0f;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int n, bool vec, const float* v)
+{
+    if (n >= 8 && vec) {
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+            *(reinterpret_cast<float4*>(p) + 1) = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+            uint4 u;
+            T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) e[j] = from_f32<T>(v[j]);
+            *reinterpret_cast<uint4*>(p) = u;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) if (j < n) p[j] = from_f32<T>(v[j]);
+    }
+}
+
+/* The same for gamma, whose type is the call's own choice (uniform branch). */
+__device__ __forceinline__ void load8_any(const void* base, int type, int64_t at, int n, bool vec, float* v)
+{
+    if (type == DECXB_F32)      load8(static_cast<const float*>(base) + at, n, vec, v);
+    else if (type == DECXB_F16) load8(static_cast<const __half*>(base) + at, n, vec, v);
+    else                        load8(static_cast<const __nv_bfloat16*>(base) + at, n, vec, v);
+}
+
+/* ------------------------------------------------------------------ codes and scales -- */
+/* NaN wins (fmaxf would drop it): a NaN in a block has to reach its scale. */
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+    float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r;
+}
+
+__device__ __forceinline__ float scale_of(float amax, int type, int rule)
+{
+    float s = __fdiv_rn(amax, type == DECXB_FP8_E4M3 ? 448.0f : 57344.0f);
+    if (rule == DECXB_SCALE_POW2) {
+        /* up to the next power of two: exponent + 1 unless the mantissa is zero (infinity and NaN stay) */
+        const uint32_t u = __float_as_uint(s);
+        if ((u & 0x7f800000u) != 0x7f800000u && (u & 0x007fffffu)) s = __uint_as_float((u & 0x7f800000u) + 0x00800000u);
+    }
+    return s < 1.17549435e-38f ? 1.17549435e-38f : s;
+}
+
+/* Eight codes of v * inv, rounded to nearest even; saturation only meets what the scale's own rounding pushed a
+ * hair over the largest value. */
+__device__ __forceinline__ uint2 codes8(const float* v, float inv, int type)
+{
+    uint32_t h[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float2 f = make_float2(v[2 * j] * inv, v[2 * j + 1] * inv);
+        h[j] = type == DECXB_FP8_E4M3 ? __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3)
+                                      : __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E5M2);
+    }
+    return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+}
+
+__device__ __forceinline__ void store_codes8(uint8_t* p, int n, bool vec, uint2 c)
+{
+    if (n >= 8 && vec) *reinterpret_cast<uint2*>(p) = c;
+    else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) if (j < n) p[j] = (uint8_t)((j < 4 ? c.x : c.y) >> (8 * (j & 3)));
+    }
+}
+
+/* ------------------------------------------------------------------ host side -------- */
+/* Makes the context's device current for one entry and puts the caller's back. */
+struct DeviceScope {
+    int prev = -1, status;
+    explicit DeviceScope(decxb_ctx* ctx)
+    {
+        if (cudaGetDevice(&prev) != cudaSuccess) { cudaGetLastError(); prev = -1; }
+        status = decxb_bind(ctx);
+        if (ctx && prev == ctx->device) prev = -1;
+    }
+    ~DeviceScope() { if (prev >= 0) cudaSetDevice(prev); }
+};
+
+inline int size_of(int type) { return type == DECXB_F32 ? 4 : 2; }
+inline bool type_ok(int type) { return type == DECXB_F32 || type == DECXB_F16 || type == DECXB_BF16; }
+inline bool aligned(const void* p, int64_t row_bytes, int to) { return (reinterpret_cast<uintptr_t>(p) % to) == 0 && row_bytes % to == 0; }
+
+/* An fp8 matrix as an argument: `rows` x `cols` (-1: any). */
+inline int check_matrix(decxb_ctx* ctx, const decxb_fp8_matrix* m, const char* name, int64_t rows, int64_t cols)
+{
+    const std::string n(name);
+    if (m->type != DECXB_FP8_E4M3 && m->type != DECXB_FP8_E5M2) return decxb_fail(ctx, DECXB_ERR_BAD_FLAG, n + ": fp8 type");
+    if (m->block_rows != 1 && m->block_rows != 128) return decxb_fail(ctx, DECXB_ERR_BAD_PARAM, n + ": block_rows must be 1 or 128");
+    if (m->rows < 0 || m->cols < 0) return decxb_fail(ctx, DECXB_ERR_BAD_PARAM, n + ": negative size");
+    if ((rows >= 0 && m->rows != rows) || (cols >= 0 && m->cols != cols)) return decxb_fail(ctx, DECXB_ERR_DIM_MISMATCH, n + ": rows or cols");
+    if (m->ld < m->cols) return decxb_fail(ctx, DECXB_ERR_DIM_MISMATCH, n + ": leading dimension smaller than the row length");
+    if (m->rows > 0x7fffffffLL || m->cols > 0x7fffffffLL) return decxb_fail(ctx, DECXB_ERR_TOO_LARGE, n + ": rows or cols");
+    if (m->scale_row_stride < 0 || m->scale_block_stride < 0) return decxb_fail(ctx, DECXB_ERR_BAD_PARAM, n + ": negative scale stride");
+    if (m->rows > 0 && m->cols > 0 && (!m->data || !m->scales)) return decxb_fail(ctx, DECXB_ERR_BAD_PARAM, n + ": null data or scales");
+    if (reinterpret_cast<uintptr_t>(m->scales) % 4) return decxb_fail(ctx, DECXB_ERR_BAD_PARAM, n + ": scales not 4-byte aligned");
+    return DECXB_OK;
+}
+
+/* As an output: its scales may not share words either. */
+inline int check_output(decxb_ctx* ctx, const decxb_fp8_matrix* m, const char* name, int64_t rows, int64_t cols)
+{
+    if (int rc = check_matrix(ctx, m, name, rows, cols)) return rc;
+    const int64_t r = decxb_ceil_div(m->rows, m->block_rows), c = decxb_ceil_div(m->cols, 128);
+    const int64_t a = m->scale_row_stride, b = m->scale_block_stride;
+    const bool apart = (r <= 1 || c <= 1) ? !((r > 1 && a == 0) || (c > 1 && b == 0)) : (b > 0 && a > (c - 1) * b) || (a > 0 && b > (r - 1) * a);
+    if (!apart) return decxb_fail(ctx, DECXB_ERR_BAD_PARAM, std::string(name) + ": scale strides make blocks share a scale");
+    return DECXB_OK;
+}
+
+/* A [rows][cols] array argument of element size `e`. */
+inline int check_array(decxb_ctx* ctx, const void* p, int64_t ld, int64_t cols, int e, const char* name)
+{
+    if (!p) return decxb_fail(ctx, DECXB_ERR_BAD_PARAM, std::string(name) + ": null");
+    if (reinterpret_cast<uintptr_t>(p) % e) return decxb_fail(ctx, DECXB_ERR_BAD_PARAM, std::string(name) + ": not aligned to its elements");
+    if (ld < cols) return decxb_fail(ctx, DECXB_ERR_DIM_MISMATCH, std::string(name) + ": leading dimension smaller than the row length");
+    return DECXB_OK;
+}
+
+/* Whether scratch may be taken on stream `s`: under capture it would outlive the call that owns it. */
+inline int refuse_capture(decxb_ctx* ctx, cudaStream_t s, const char* what)
+{
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    const cudaError_t e = cudaStreamIsCapturing(s, &st);
+    if (e != cudaSuccess) cudaGetLastError();
+    if (e != cudaSuccess || st != cudaStreamCaptureStatusNone)
+        return decxb_fail(ctx, DECXB_ERR_BAD_PARAM, std::string("the stream is being captured and ") + what);
+    return DECXB_OK;
+}
+
+}  // namespace fp8
+#endif

@@ -1,0 +1,618 @@
+/*
+ * What feeds the 8-bit product (sm_100a): quantisation of a matrix as it stands and transposed, the
+ * root-mean-square norm with the residual's addition and an fp8 output, and the norm's backward pass.
+ * All of them are bound by memory: every array is read once and written once.
+ */
+#include "fp8.cuh"
+
+#include <new>
+
+namespace {
+
+using namespace fp8;
+
+__device__ __forceinline__ float warp_sum(float v)
+{
+#pragma unroll
+    for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+/* ---- root-mean-square norm ---------------------------------------------------------------
+ * One block per row.  A thread holds VPT vectors of eight consecutive columns, vector i * blockDim + tid, so the
+ * 16 lanes of half a warp cover one 128-column block of the row and its largest magnitude is four shuffles away. */
+struct NormArgs {
+    int64_t rows, cols;
+    const void *x, *r, *gamma; void *h, *y;
+    int64_t ldx, ldr, ldh, ldy;
+    int gamma_type, rule;
+    float eps;
+    bool vec, gvec;                   /* 128-bit accesses to x, r, h, y / gamma                     */
+    uint8_t* q; int64_t ldq; float* s; int64_t srs, sbs; int qtype; bool qvec;
+};
+
+/* Quantises eight columns from `c` on of one row: the 16 lanes of the block agree on its scale. */
+__device__ __forceinline__ void quantise_row8(const NormArgs& a, int64_t row, int64_t c, const float* y)
+{
+    const int n = (int)min((int64_t)8, a.cols - c);
+    float amax = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) amax = max_nan(amax, j < n ? fabsf(y[j]) : 0.0f);
+#pragma unroll
+    for (int o = 8; o; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if (n <= 0) return;
+    const float s = scale_of(amax, a.qtype, a.rule);
+    store_codes8(a.q + row * a.ldq + c, n, a.qvec, codes8(y, __frcp_rn(s), a.qtype));
+    if ((c & 127) == 0) a.s[row * a.srs + (c >> 7) * a.sbs] = s;
+}
+
+template <typename T, int VPT>
+__global__ void __launch_bounds__(1024)
+decxb_rmsnorm_kernel(const NormArgs a)
+{
+    __shared__ float part[32];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nwarps = blockDim.x >> 5;
+    const int64_t row = blockIdx.x;
+    const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+    const T* r = a.r ? static_cast<const T*>(a.r) + row * a.ldr : nullptr;
+    float v[VPT][8];
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        const int64_t c = ((int64_t)i * blockDim.x + tid) * 8;
+        const int n = (int)min((int64_t)8, a.cols - c);
+        load8(x + c, n, a.vec, v[i]);
+        if (r) {
+            float w[8];
+            load8(r + c, n, a.vec, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] += w[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum = fmaf(v[i][j], v[i][j], sum);
+    }
+    sum = warp_sum(sum);
+    if (nwarps > 1) {
+        if (lane == 0) part[warp] = sum;
+        __syncthreads();
+        sum = warp_sum(lane < nwarps ? part[lane] : 0.0f);
+    }
+    const float rstd = rsqrtf(sum / (float)a.cols + a.eps);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        const int64_t c = ((int64_t)i * blockDim.x + tid) * 8;
+        const int n = (int)min((int64_t)8, a.cols - c);
+        if (a.h && n > 0) store8(static_cast<T*>(a.h) + row * a.ldh + c, n, a.vec, v[i]);
+        float g[8];
+        load8_any(a.gamma, a.gamma_type, c, n, a.gvec, g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * rstd * g[j];
+        if (a.y && n > 0) store8(static_cast<T*>(a.y) + row * a.ldy + c, n, a.vec, v[i]);
+        if (a.q) quantise_row8(a, row, c, v[i]);
+    }
+}
+
+/* Rows too long for the registers: the row is read twice (the second time from L2, mostly). */
+template <typename T>
+__global__ void __launch_bounds__(1024)
+decxb_rmsnorm_wide_kernel(const NormArgs a)
+{
+    __shared__ float part[32];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nwarps = blockDim.x >> 5;
+    const int64_t row = blockIdx.x;
+    const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+    const T* r = a.r ? static_cast<const T*>(a.r) + row * a.ldr : nullptr;
+    float sum = 0.0f, v[8], w[8];
+    for (int64_t c = (int64_t)tid * 8; c < a.cols; c += (int64_t)blockDim.x * 8) {
+        const int n = (int)min((int64_t)8, a.cols - c);
+        load8(x + c, n, a.vec, v);
+        if (r) {
+            load8(r + c, n, a.vec, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] += w[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum = fmaf(v[j], v[j], sum);
+    }
+    sum = warp_sum(sum);
+    if (lane == 0) part[warp] = sum;
+    __syncthreads();
+    sum = warp_sum(lane < nwarps ? part[lane] : 0.0f);
+    const float rstd = rsqrtf(sum / (float)a.cols + a.eps);
+    /* whole warps go round together (the quantisation exchanges values inside a warp) */
+    for (int64_t c0 = (int64_t)warp * 256; c0 < a.cols; c0 += (int64_t)blockDim.x * 8) {
+        const int64_t c = c0 + lane * 8;
+        const int n = (int)min((int64_t)8, a.cols - c);
+        load8(x + c, n, a.vec, v);
+        if (r) {
+            load8(r + c, n, a.vec, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] += w[j];
+        }
+        if (a.h && n > 0) store8(static_cast<T*>(a.h) + row * a.ldh + c, n, a.vec, v);
+        load8_any(a.gamma, a.gamma_type, c, n, a.gvec, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = v[j] * rstd * w[j];
+        if (a.y && n > 0) store8(static_cast<T*>(a.y) + row * a.ldy + c, n, a.vec, v);
+        if (a.q) quantise_row8(a, row, c, v);
+    }
+}
+
+/* Threads per row: multiples of 32 that cover `nvec` vectors with at most `vpt` each. */
+int threads_for(int64_t nvec, int vpt, int most)
+{
+    int64_t t = decxb_ceil_to(decxb_ceil_div(nvec, vpt), 32);
+    return (int)(t > most ? most : t < 32 ? 32 : t);
+}
+
+template <typename T>
+int launch_norm(decxb_ctx* ctx, const NormArgs& a, cudaStream_t s)
+{
+    const int64_t nvec = decxb_ceil_div(a.cols, 8);
+    decxb_launch_scope scope(ctx, s, DECXB_K_SPLIT);
+    const unsigned grid = (unsigned)a.rows;
+    if (nvec <= 512)       decxb_rmsnorm_kernel<T, 1><<<grid, threads_for(nvec, 1, 512), 0, s>>>(a);
+    else if (nvec <= 1024) decxb_rmsnorm_kernel<T, 2><<<grid, threads_for(nvec, 2, 512), 0, s>>>(a);
+    else if (nvec <= 4096) decxb_rmsnorm_kernel<T, 4><<<grid, threads_for(nvec, 4, 1024), 0, s>>>(a);
+    else                   decxb_rmsnorm_wide_kernel<T><<<grid, 1024, 0, s>>>(a);
+    DECXB_CUDA_TRY(ctx, cudaGetLastError());
+    return DECXB_OK;
+}
+
+/* ---- its backward pass ---------------------------------------------------------------------
+ * A block walks rows blockIdx, blockIdx + gridDim, ...; a thread keeps the same columns throughout and sums their share
+ * of dgamma in registers.  Each block leaves its sums in its own row of the workspace, and a second kernel adds
+ * the rows in ascending order: no atomics, the same bits every time. */
+struct NormBwdArgs {
+    int64_t rows, cols;
+    const void *dy, *h, *dr, *gamma; void* dx;
+    int64_t lddy, ldh, lddr, lddx;
+    int gamma_type;
+    float eps;
+    bool vec, gvec;
+    float* part;                      /* [gridDim][cols], or NULL                                    */
+};
+
+/* Sums of (a, b) over the block; `buf` alternates between rows so that one barrier a row is enough. */
+__device__ __forceinline__ float2 block_sum2(float a, float b, float2* buf, int warp, int lane, int nwarps)
+{
+    a = warp_sum(a); b = warp_sum(b);
+    if (nwarps == 1) return make_float2(a, b);
+    if (lane == 0) buf[warp] = make_float2(a, b);
+    __syncthreads();
+    const float2 p = lane < nwarps ? buf[lane] : make_float2(0.0f, 0.0f);
+    return make_float2(warp_sum(p.x), warp_sum(p.y));
+}
+
+template <typename T, int VPT>
+__global__ void __launch_bounds__(512)
+decxb_rmsnorm_backward_kernel(const NormBwdArgs a)
+{
+    __shared__ float2 buf[2][32];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nwarps = blockDim.x >> 5;
+    float acc[VPT][8];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[i][j] = 0.0f;
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+        const T* dy = static_cast<const T*>(a.dy) + row * a.lddy;
+        const T* h = static_cast<const T*>(a.h) + row * a.ldh;
+        float w[VPT][8], x[VPT][8];
+        float sq = 0.0f, dot = 0.0f;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int64_t c = ((int64_t)i * blockDim.x + tid) * 8;
+            const int n = (int)min((int64_t)8, a.cols - c);
+            load8(dy + c, n, a.vec, w[i]);
+            load8(h + c, n, a.vec, x[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int64_t c = ((int64_t)i * blockDim.x + tid) * 8;
+            const int n = (int)min((int64_t)8, a.cols - c);
+            float g[8];
+            load8_any(a.gamma, a.gamma_type, c, n, a.gvec, g);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                sq = fmaf(x[i][j], x[i][j], sq);
+                dot = fmaf(w[i][j] * g[j], x[i][j], dot);
+            }
+        }
+        const float2 s = block_sum2(sq, dot, buf[turn], warp, lane, nwarps);
+        const float r = rsqrtf(s.x / (float)a.cols + a.eps);
+        const float k = r * r * (s.y / (float)a.cols);
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int64_t c = ((int64_t)i * blockDim.x + tid) * 8;
+            const int n = (int)min((int64_t)8, a.cols - c);
+            if (n <= 0) continue;
+            float g[8], o[8];
+            load8_any(a.gamma, a.gamma_type, c, n, a.gvec, g);
+            if (a.dr) load8(static_cast<const T*>(a.dr) + row * a.lddr + c, n, a.vec, o);
+            else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) o[j] = 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                acc[i][j] = fmaf(w[i][j], x[i][j] * r, acc[i][j]);
+                o[j] = fmaf(r, w[i][j] * g[j] - x[i][j] * k, o[j]);
+            }
+            store8(static_cast<T*>(a.dx) + row * a.lddx + c, n, a.vec, o);
+        }
+    }
+    if (!a.part) return;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        const int64_t c = ((int64_t)i * blockDim.x + tid) * 8;
+        const int n = (int)min((int64_t)8, a.cols - c);
+        if (n > 0) store8(a.part + (int64_t)blockIdx.x * a.cols + c, n, a.cols % 4 == 0, acc[i]);
+    }
+}
+
+/* Rows too long for the registers: each row is read twice and the sums for dgamma live in the workspace. */
+template <typename T>
+__global__ void __launch_bounds__(512)
+decxb_rmsnorm_backward_wide_kernel(const NormBwdArgs a)
+{
+    __shared__ float2 buf[2][32];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nwarps = blockDim.x >> 5;
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+        const T* dy = static_cast<const T*>(a.dy) + row * a.lddy;
+        const T* h = static_cast<const T*>(a.h) + row * a.ldh;
+        float sq = 0.0f, dot = 0.0f, w[8], x[8], g[8], o[8];
+        for (int64_t c = (int64_t)tid * 8; c < a.cols; c += (int64_t)blockDim.x * 8) {
+            const int n = (int)min((int64_t)8, a.cols - c);
+            load8(dy + c, n, a.vec, w); load8(h + c, n, a.vec, x); load8_any(a.gamma, a.gamma_type, c, n, a.gvec, g);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { sq = fmaf(x[j], x[j], sq); dot = fmaf(w[j] * g[j], x[j], dot); }
+        }
+        const float2 s = block_sum2(sq, dot, buf[turn], warp, lane, nwarps);
+        const float r = rsqrtf(s.x / (float)a.cols + a.eps);
+        const float k = r * r * (s.y / (float)a.cols);
+        for (int64_t c = (int64_t)tid * 8; c < a.cols; c += (int64_t)blockDim.x * 8) {
+            const int n = (int)min((int64_t)8, a.cols - c);
+            load8(dy + c, n, a.vec, w); load8(h + c, n, a.vec, x); load8_any(a.gamma, a.gamma_type, c, n, a.gvec, g);
+            if (a.dr) load8(static_cast<const T*>(a.dr) + row * a.lddr + c, n, a.vec, o);
+            else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) o[j] = 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j] = fmaf(r, w[j] * g[j] - x[j] * k, o[j]);
+            if (a.part) {
+                float* p = a.part + (int64_t)blockIdx.x * a.cols + c;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (j < n) p[j] = fmaf(w[j], x[j] * r, row == (int64_t)blockIdx.x ? 0.0f : p[j]);
+            }
+            store8(static_cast<T*>(a.dx) + row * a.lddx + c, n, a.vec, o);
+        }
+    }
+}
+
+/* dgamma[c] = sum over the workspace's rows: 32 columns a block, 32 groups of rows side by side. */
+__global__ void __launch_bounds__(1024)
+decxb_column_sum_kernel(const float* __restrict__ part, int parts, int64_t cols, float* __restrict__ out)
+{
+    __shared__ float sums[32][33];
+    const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+    float v = 0.0f;
+    if (c < cols)
+        for (int p = group; p < parts; p += 32) v += part[(int64_t)p * cols + c];
+    sums[group][lane] = v;
+    __syncthreads();
+    v = warp_sum(sums[lane][group]);            /* warp g adds the 32 groups of column g */
+    const int64_t co = (int64_t)blockIdx.x * 32 + group;
+    if (lane == 0 && co < cols) out[co] = v;
+}
+
+/* Blocks of the backward kernel = rows of its workspace. */
+int64_t backward_blocks(const decxb_ctx* ctx, int64_t rows)
+{
+    const int64_t most = (int64_t)ctx->sm_count * 2;
+    return rows < most ? rows : most;
+}
+
+template <typename T>
+int launch_norm_backward(decxb_ctx* ctx, const NormBwdArgs& a, float* dgamma, cudaStream_t s)
+{
+    const int64_t nvec = decxb_ceil_div(a.cols, 8);
+    const unsigned grid = (unsigned)backward_blocks(ctx, a.rows);
+    {
+        decxb_launch_scope scope(ctx, s, DECXB_K_SPLIT);
+        if (nvec <= 512)       decxb_rmsnorm_backward_kernel<T, 1><<<grid, threads_for(nvec, 1, 512), 0, s>>>(a);
+        else if (nvec <= 1024) decxb_rmsnorm_backward_kernel<T, 2><<<grid, threads_for(nvec, 2, 512), 0, s>>>(a);
+        else if (nvec <= 2048) decxb_rmsnorm_backward_kernel<T, 4><<<grid, threads_for(nvec, 4, 512), 0, s>>>(a);
+        else                   decxb_rmsnorm_backward_wide_kernel<T><<<grid, 512, 0, s>>>(a);
+        DECXB_CUDA_TRY(ctx, cudaGetLastError());
+    }
+    if (dgamma) {
+        decxb_launch_scope scope(ctx, s, DECXB_K_SPLIT);
+        decxb_column_sum_kernel<<<(unsigned)decxb_ceil_div(a.cols, 32), 1024, 0, s>>>(a.part, (int)grid, a.cols, dgamma);
+        DECXB_CUDA_TRY(ctx, cudaGetLastError());
+    }
+    return DECXB_OK;
+}
+
+/* ---- quantisation -------------------------------------------------------------------------
+ * A block of 256 threads holds one 128 x 128 tile of X in registers: thread (g, t) = (tid / 16, tid % 16) has rows
+ * 8 g .. 8 g + 7 of columns 8 t .. 8 t + 7.  A row's 128 values lie in the 16 lanes of half a warp; a column's in
+ * the 16 groups, which meet through shared memory.  The transposed codes leave through shared memory as well,
+ * eight rows (8 bytes) of a column at a time, the 8-byte pieces of a column XOR-ed with the column group so that
+ * the 16 lanes of a store fall into 16 different bank pairs. */
+struct QuantArgs {
+    int64_t rows, cols, ldx;
+    const void* x;
+    int rule; bool vec;
+    int64_t tiles_c;
+    struct Out { uint8_t* data; float* s; int64_t ld, srs, sbs; int type, block_rows; bool vec; } q, t;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+decxb_quantize_fp8_kernel(const QuantArgs a)
+{
+    __shared__ float colmax[8][128];
+    __shared__ float wmax[8];
+    __shared__ __align__(16) uint8_t tr[128 * 128];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = tid >> 4, t = tid & 15;
+    const int64_t tile_r = blockIdx.x / a.tiles_c, tile_c = blockIdx.x % a.tiles_c;
+    const int64_t r0 = tile_r * 128, c0 = tile_c * 128;
+    const int64_t row = r0 + g * 8, col = c0 + t * 8;
+    const int nr = (int)max((int64_t)0, min((int64_t)8, a.rows - row));          /* rows and columns that exist here */
+    const int nc = (int)max((int64_t)0, min((int64_t)8, a.cols - col));
+    float v[8][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        load8(static_cast<const T*>(a.x) + (row + i) * a.ldx + col, i < nr ? nc : 0, a.vec, v[i]);
+
+    const bool whole = (a.q.data && a.q.block_rows == 128) || (a.t.data && a.t.block_rows == 128);
+    const bool by_col = a.t.data && a.t.block_rows == 1;
+    if (whole || by_col) {
+        float m8[8], m = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            m8[j] = fabsf(v[0][j]);
+#pragma unroll
+            for (int i = 1; i < 8; ++i) m8[j] = max_nan(m8[j], fabsf(v[i][j]));
+            m8[j] = max_nan(m8[j], __shfl_xor_sync(0xffffffffu, m8[j], 16));
+            m = max_nan(m, m8[j]);
+        }
+        if (by_col && lane < 16) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) colmax[warp][t * 8 + j] = m8[j];
+        }
+#pragma unroll
+        for (int o = 8; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (lane == 0) wmax[warp] = m;
+        __syncthreads();
+    }
+    float tile_max = 0.0f;
+    if (whole) {
+#pragma unroll
+        for (int w = 0; w < 8; ++w) tile_max = max_nan(tile_max, wmax[w]);
+    }
+
+    if (a.q.data) {
+        const float st = a.q.block_rows == 128 ? scale_of(tile_max, a.q.type, a.rule) : 0.0f;
+        if (a.q.block_rows == 128 && tid == 0) a.q.s[tile_r * a.q.srs + tile_c * a.q.sbs] = st;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float s = st;
+            if (a.q.block_rows == 1) {
+                float m = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(v[i][j]));
+#pragma unroll
+                for (int o = 8; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+                s = scale_of(m, a.q.type, a.rule);
+                if (t == 0 && i < nr) a.q.s[(row + i) * a.q.srs + tile_c * a.q.sbs] = s;
+            }
+            if (i < nr && nc > 0) store_codes8(a.q.data + (row + i) * a.q.ld + col, nc, a.q.vec, codes8(v[i], __frcp_rn(s), a.q.type));
+        }
+    }
+
+    if (a.t.data) {
+        const float st = a.t.block_rows == 128 ? scale_of(tile_max, a.t.type, a.rule) : 0.0f;
+        if (a.t.block_rows == 128 && tid == 0) a.t.s[tile_c * a.t.srs + tile_r * a.t.sbs] = st;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float s = st;
+            if (by_col) {
+                float m = 0.0f;
+#pragma unroll
+                for (int w = 0; w < 8; ++w) m = max_nan(m, colmax[w][t * 8 + j]);
+                s = scale_of(m, a.t.type, a.rule);
+                if (g == 0 && j < nc) a.t.s[(col + j) * a.t.srs + tile_r * a.t.sbs] = s;
+            }
+            float w8[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w8[i] = v[i][j];
+            *reinterpret_cast<uint2*>(tr + (t * 8 + j) * 128 + ((g ^ t) << 3)) = codes8(w8, __frcp_rn(s), a.t.type);
+        }
+        __syncthreads();
+        /* out: row c of the transpose, eight of X's rows per thread, 16 lanes a row */
+        const int nro = (int)max((int64_t)0, min((int64_t)8, a.rows - (r0 + t * 8)));
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+            const int c = p * 16 + g;
+            const uint2 k = *reinterpret_cast<const uint2*>(tr + c * 128 + ((t ^ (c >> 3)) << 3));
+            if (c0 + c < a.cols && nro > 0) store_codes8(a.t.data + (c0 + c) * a.t.ld + r0 + t * 8, nro, a.t.vec, k);
+        }
+    }
+}
+
+template <typename T>
+int launch_quantize(decxb_ctx* ctx, const QuantArgs& a, cudaStream_t s)
+{
+    const int64_t tiles = decxb_ceil_div(a.rows, 128) * a.tiles_c;
+    if (tiles > 0x7fffffffLL) return decxb_fail(ctx, DECXB_ERR_TOO_LARGE, "tiles of 128 x 128");
+    decxb_launch_scope scope(ctx, s, DECXB_K_SPLIT);
+    decxb_quantize_fp8_kernel<T><<<(unsigned)tiles, 256, 0, s>>>(a);
+    DECXB_CUDA_TRY(ctx, cudaGetLastError());
+    return DECXB_OK;
+}
+
+QuantArgs::Out out_of(const decxb_fp8_matrix* m)
+{
+    if (!m) return {};
+    return {static_cast<uint8_t*>(m->data), m->scales, m->ld, m->scale_row_stride, m->scale_block_stride, m->type, m->block_rows,
+            aligned(m->data, m->ld, 8)};
+}
+
+int quantize(decxb_ctx* ctx, int x_type, int64_t rows, int64_t cols, const void* X, int64_t ldx, int rule,
+             const decxb_fp8_matrix* Q, const decxb_fp8_matrix* Qt, cudaStream_t s)
+{
+    if (!type_ok(x_type)) return decxb_fail(ctx, DECXB_ERR_BAD_FLAG, "x_type");
+    if (rule != DECXB_SCALE_AMAX && rule != DECXB_SCALE_POW2) return decxb_fail(ctx, DECXB_ERR_BAD_FLAG, "scale rule");
+    if (rows < 0 || cols < 0) return decxb_fail(ctx, DECXB_ERR_BAD_PARAM, "negative size");
+    if (!Q && !Qt) return decxb_fail(ctx, DECXB_ERR_BAD_PARAM, "nothing to write");
+    int rc;
+    if (Q && (rc = check_output(ctx, Q, "Q", rows, cols))) return rc;
+    if (Qt && (rc = check_output(ctx, Qt, "Qt", cols, rows))) return rc;
+    if (rows == 0 || cols == 0) return DECXB_OK;
+    if ((rc = check_array(ctx, X, ldx, cols, size_of(x_type), "X"))) return rc;
+    QuantArgs a = {};
+    a.rows = rows; a.cols = cols; a.x = X; a.ldx = ldx; a.rule = rule;
+    a.vec = aligned(X, ldx * size_of(x_type), 16);
+    a.tiles_c = decxb_ceil_div(cols, 128);
+    a.q = out_of(Q); a.t = out_of(Qt);
+    if (x_type == DECXB_F32) return launch_quantize<float>(ctx, a, s);
+    if (x_type == DECXB_F16) return launch_quantize<__half>(ctx, a, s);
+    return launch_quantize<__nv_bfloat16>(ctx, a, s);
+}
+
+int norm_common(decxb_ctx* ctx, int type, int64_t rows, int64_t cols, int gamma_type, float eps)
+{
+    if (!type_ok(type) || !type_ok(gamma_type)) return decxb_fail(ctx, DECXB_ERR_BAD_FLAG, "type");
+    if (rows < 0 || cols <= 0) return decxb_fail(ctx, DECXB_ERR_BAD_PARAM, "rows must not be negative, cols must be positive");
+    if (rows > 0x7fffffffLL || cols > 0x7fffffffLL) return decxb_fail(ctx, DECXB_ERR_TOO_LARGE, "rows or cols");
+    if (!(eps >= 0.0f) || eps > 3.0e38f) return decxb_fail(ctx, DECXB_ERR_BAD_PARAM, "eps must be a finite number >= 0");
+    return DECXB_OK;
+}
+
+int norm(decxb_ctx* ctx, int type, int64_t rows, int64_t cols, const void* X, int64_t ldx, const void* R, int64_t ldr,
+         const void* gamma, int gamma_type, float eps, void* H, int64_t ldh, void* Y, int64_t ldy, int rule,
+         const decxb_fp8_matrix* Q, cudaStream_t s)
+{
+    int rc = norm_common(ctx, type, rows, cols, gamma_type, eps);
+    if (rc) return rc;
+    if (rule != DECXB_SCALE_AMAX && rule != DECXB_SCALE_POW2) return decxb_fail(ctx, DECXB_ERR_BAD_FLAG, "scale rule");
+    if (!H && !Y && !Q) return decxb_fail(ctx, DECXB_ERR_BAD_PARAM, "nothing to write");
+    if (Q && (rc = check_output(ctx, Q, "Q", rows, cols))) return rc;
+    if (Q && Q->block_rows != 1) return decxb_fail(ctx, DECXB_ERR_BAD_PARAM, "Q: block_rows must be 1");
+    if (rows == 0) return DECXB_OK;
+    const int e = size_of(type);
+    if ((rc = check_array(ctx, X, ldx, cols, e, "X")) || (rc = check_array(ctx, gamma, cols, cols, size_of(gamma_type), "gamma"))) return rc;
+    if (R && (rc = check_array(ctx, R, ldr, cols, e, "R"))) return rc;
+    if (H && (rc = check_array(ctx, H, ldh, cols, e, "H"))) return rc;
+    if (Y && (rc = check_array(ctx, Y, ldy, cols, e, "Y"))) return rc;
+    if (H && H == Y) return decxb_fail(ctx, DECXB_ERR_BAD_PARAM, "H and Y are the same array");
+    if ((H == X && H && ldh != ldx) || (H == R && H && ldh != ldr) || (Y == X && Y && ldy != ldx) || (Y == R && Y && ldy != ldr))
+        return decxb_fail(ctx, DECXB_ERR_BAD_PARAM, "an output in place of an input needs its leading dimension");
+    NormArgs a = {};
+    a.rows = rows; a.cols = cols; a.x = X; a.r = R; a.gamma = gamma; a.h = H; a.y = Y;
+    a.ldx = ldx; a.ldr = ldr; a.ldh = ldh; a.ldy = ldy; a.gamma_type = gamma_type; a.rule = rule; a.eps = eps;
+    a.vec = aligned(X, ldx * e, 16) && (!R || aligned(R, ldr * e, 16)) && (!H || aligned(H, ldh * e, 16)) && (!Y || aligned(Y, ldy * e, 16));
+    a.gvec = aligned(gamma, 0, 16);
+    if (Q) {
+        a.q = static_cast<uint8_t*>(Q->data); a.ldq = Q->ld; a.s = Q->scales; a.srs = Q->scale_row_stride; a.sbs = Q->scale_block_stride;
+        a.qtype = Q->type; a.qvec = aligned(Q->data, Q->ld, 8);
+    }
+    if (type == DECXB_F32) return launch_norm<float>(ctx, a, s);
+    if (type == DECXB_F16) return launch_norm<__half>(ctx, a, s);
+    return launch_norm<__nv_bfloat16>(ctx, a, s);
+}
+
+size_t backward_bytes(const decxb_ctx* ctx, int64_t rows, int64_t cols)
+{
+    return (size_t)backward_blocks(ctx, rows) * (size_t)cols * sizeof(float);
+}
+
+int norm_backward(decxb_ctx* ctx, int type, int64_t rows, int64_t cols, const void* dY, int64_t lddy, const void* H, int64_t ldh,
+                  const void* gamma, int gamma_type, float eps, const void* dR, int64_t lddr, void* dX, int64_t lddx, float* dgamma,
+                  void* workspace, size_t workspace_bytes, cudaStream_t s)
+{
+    int rc = norm_common(ctx, type, rows, cols, gamma_type, eps);
+    if (rc) return rc;
+    if (reinterpret_cast<uintptr_t>(dgamma) % 4) return decxb_fail(ctx, DECXB_ERR_BAD_PARAM, "dgamma: not aligned to its elements");
+    if (rows == 0) {
+        if (dgamma) DECXB_CUDA_TRY(ctx, cudaMemsetAsync(dgamma, 0, (size_t)cols * sizeof(float), s));
+        return DECXB_OK;
+    }
+    const int e = size_of(type);
+    if ((rc = check_array(ctx, dY, lddy, cols, e, "dY")) || (rc = check_array(ctx, H, ldh, cols, e, "H")) ||
+        (rc = check_array(ctx, gamma, cols, cols, size_of(gamma_type), "gamma")) || (rc = check_array(ctx, dX, lddx, cols, e, "dX"))) return rc;
+    if (dR && (rc = check_array(ctx, dR, lddr, cols, e, "dR"))) return rc;
+    if ((dX == dY && lddx != lddy) || (dX == dR && lddx != lddr))
+        return decxb_fail(ctx, DECXB_ERR_BAD_PARAM, "dX in place of an input needs its leading dimension");
+    if (dX == H) return decxb_fail(ctx, DECXB_ERR_BAD_PARAM, "dX may not be H");
+    const size_t need = dgamma ? backward_bytes(ctx, rows, cols) : 0;
+    NormBwdArgs a = {};
+    a.rows = rows; a.cols = cols; a.dy = dY; a.h = H; a.dr = dR; a.gamma = gamma; a.dx = dX;
+    a.lddy = lddy; a.ldh = ldh; a.lddr = lddr; a.lddx = lddx; a.gamma_type = gamma_type; a.eps = eps;
+    a.vec = aligned(dY, lddy * e, 16) && aligned(H, ldh * e, 16) && (!dR || aligned(dR, lddr * e, 16)) && aligned(dX, lddx * e, 16);
+    a.gvec = aligned(gamma, 0, 16);
+    void* scratch = nullptr;
+    if (need && workspace) {
+        if (workspace_bytes < need) return decxb_fail(ctx, DECXB_ERR_BAD_PARAM, "workspace of " + std::to_string(need) + " bytes needed");
+        if (reinterpret_cast<uintptr_t>(workspace) % 16) return decxb_fail(ctx, DECXB_ERR_BAD_PARAM, "workspace not 16-byte aligned");
+        a.part = static_cast<float*>(workspace);
+    } else if (need) {
+        if ((rc = refuse_capture(ctx, s, "no workspace was given"))) return rc;
+        if ((rc = decxb_malloc_on_stream(ctx, need, &scratch, s))) return rc;
+        a.part = static_cast<float*>(scratch);
+    }
+    rc = type == DECXB_F32 ? launch_norm_backward<float>(ctx, a, dgamma, s)
+       : type == DECXB_F16 ? launch_norm_backward<__half>(ctx, a, dgamma, s)
+                           : launch_norm_backward<__nv_bfloat16>(ctx, a, dgamma, s);
+    if (scratch) decxb_free_on_stream(ctx, scratch, s);
+    return rc;
+}
+
+cudaStream_t stream_of(decxb_ctx* ctx, void* stream) { return stream ? (cudaStream_t)stream : ctx->stream; }
+
+}  // namespace
+
+extern "C" int decxb_quantize_fp8(decxb_ctx* ctx, int x_type, int64_t rows, int64_t cols, const void* X, int64_t ldx,
+                                  int scale_rule, const decxb_fp8_matrix* Q, const decxb_fp8_matrix* Qt, void* stream)
+try {
+    DeviceScope dev(ctx);
+    if (dev.status) return dev.status;
+    return quantize(ctx, x_type, rows, cols, X, ldx, scale_rule, Q, Qt, stream_of(ctx, stream));
+} catch (const std::bad_alloc&) { return DECXB_ERR_ALLOC; }
+
+extern "C" int decxb_rmsnorm(decxb_ctx* ctx, int type, int64_t rows, int64_t cols, const void* X, int64_t ldx,
+                             const void* R, int64_t ldr, const void* gamma, int gamma_type, float eps,
+                             void* H, int64_t ldh, void* Y, int64_t ldy,
+                             int scale_rule, const decxb_fp8_matrix* Q, void* stream)
+try {
+    DeviceScope dev(ctx);
+    if (dev.status) return dev.status;
+    return norm(ctx, type, rows, cols, X, ldx, R, ldr, gamma, gamma_type, eps, H, ldh, Y, ldy, scale_rule, Q, stream_of(ctx, stream));
+} catch (const std::bad_alloc&) { return DECXB_ERR_ALLOC; }
+
+extern "C" int decxb_rmsnorm_backward_workspace(decxb_ctx* ctx, int64_t rows, int64_t cols, size_t* bytes)
+{
+    if (!ctx || ctx->device < 0) return DECXB_ERR_NOT_INIT;
+    if (!bytes || rows < 0 || cols < 0) return DECXB_ERR_BAD_PARAM;
+    *bytes = backward_bytes(ctx, rows, cols);
+    return DECXB_OK;
+}
+
+extern "C" int decxb_rmsnorm_backward(decxb_ctx* ctx, int type, int64_t rows, int64_t cols,
+                                      const void* dY, int64_t lddy, const void* H, int64_t ldh,
+                                      const void* gamma, int gamma_type, float eps,
+                                      const void* dR, int64_t lddr, void* dX, int64_t lddx, float* dgamma,
+                                      void* workspace, size_t workspace_bytes, void* stream)
+try {
+    DeviceScope dev(ctx);
+    if (dev.status) return dev.status;
+    return norm_backward(ctx, type, rows, cols, dY, lddy, H, ldh, gamma, gamma_type, eps, dR, lddr, dX, lddx, dgamma, workspace,
+                         workspace_bytes, stream_of(ctx, stream));
+} catch (const std::bad_alloc&) { return DECXB_ERR_ALLOC; }

@@ -10,6 +10,9 @@ TILE_AUTO, TILE_1CTA_128x128, TILE_2CTA_256x256, TILE_1CTA_128x256, TILE_1CTA_12
 CONV_NO_COMPENSATE, CONV_ZERO_COMPENSATE = 0, 1
 CONV_EXPLICIT, CONV_IMPLICIT = 0, 1
 ACT_NONE, ACT_RELU, ACT_SIGMOID, ACT_TANH = 0, 1, 2, 3
+F32, F16, BF16 = 0, 1, 2
+FP8_E4M3, FP8_E5M2 = 0, 1
+SCALE_AMAX, SCALE_POW2 = 0, 1
 
 _PKG = Path(__file__).resolve().parent
 
@@ -45,6 +48,12 @@ class Profile(C.Structure):
         return {n: {"ms": self.ms[i], "launches": int(self.launches[i])} for i, n in enumerate(names)}
 
 
+class Fp8MatrixStruct(C.Structure):
+    """decxb_fp8_matrix."""
+    _fields_ = [("data", C.c_void_p), ("scales", C.c_void_p), ("rows", C.c_int64), ("cols", C.c_int64), ("ld", C.c_int64),
+                ("scale_row_stride", C.c_int64), ("scale_block_stride", C.c_int64), ("type", C.c_int32), ("block_rows", C.c_int32)]
+
+
 class TensorProbe(C.Structure):
     _fields_ = [("ms", C.c_double), ("tensor_tflops", C.c_double), ("algorithmic_tflops", C.c_double),
                 ("iterations", C.c_int64), ("sms", C.c_int)]
@@ -78,6 +87,12 @@ SIGNATURES = {
     "decxb_gemm_f32_host": (_i, [_vp, _i, _i, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64]),
     "decxb_gemm_f16": (_i, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
     "decxb_gemm_f16_host": (_i, [_vp, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64]),
+    "decxb_gemm_fp8": (_i, [_vp, _vp, _vp, _vp, _i64, _vp, _i, _i64, _vp]),
+    "decxb_quantize_fp8": (_i, [_vp, _i, _i64, _i64, _vp, _i64, _i, _vp, _vp, _vp]),
+    "decxb_rmsnorm": (_i, [_vp, _i, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i, C.c_float, _vp, _i64, _vp, _i64, _i, _vp, _vp]),
+    "decxb_rmsnorm_backward_workspace": (_i, [_vp, _i64, _i64, C.POINTER(_sz)]),
+    "decxb_rmsnorm_backward": (_i, [_vp, _i, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i, C.c_float, _vp, _i64, _vp, _i64, _vp,
+                                    _vp, _sz, _vp]),
     "decxb_gemm_f32_batched": (_i, [_vp, _i, _i, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp]),
     "decxb_gemm_f32_batched_host": (_i, [_vp, _i, _i, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64]),
     "decxb_gemm_f32_noalloc": (_i, [_i, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, C.c_char_p, _sz]),
@@ -170,6 +185,73 @@ def _ptr(x):
     raise TypeError(type(x))
 
 
+_DTYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16,
+           "float32": F32, "float16": F16}
+_FP8_TYPES = {"torch.float8_e4m3fn": FP8_E4M3, "torch.float8_e5m2": FP8_E5M2}
+
+
+def _dtype(x, given):
+    """F32 / F16 / BF16 of an array argument; `given` (needed for raw addresses) has to agree with a tensor's own."""
+    own = _DTYPES.get(str(getattr(x, "dtype", "")))
+    if own is None and given is None:
+        raise TypeError(f"element type of {type(x).__name__} {getattr(x, 'dtype', '')} is not F32, F16 or BF16: pass it")
+    if own is not None and given is not None and own != given:
+        raise TypeError(f"element type {given} given for an array of {x.dtype}")
+    return own if given is None else given
+
+
+def _stream(stream):
+    """Raw handle of a `stream` argument: None (the context's own stream), an address, or a torch stream.  Torch's default
+    stream has the address 0, which the C ABI reads as the context's own; it is passed by its explicit handle, 1."""
+    if stream is None or isinstance(stream, int):
+        return stream
+    return stream.cuda_stream or 1
+
+
+class Fp8Matrix:
+    """An fp8 matrix with a scale for each block of block_rows x 128 codes (decxb_fp8_matrix): codes [rows][cols] with
+    row pitch `ld`, scale of element (r, c) at (r // block_rows) * scale_row_stride + (c // 128) * scale_block_stride."""
+
+    def __init__(self, data, scales, rows, cols, ld, scale_row_stride, scale_block_stride, block_rows=1, type=FP8_E4M3):
+        self.data, self.scales = data, scales          # kept alive with the descriptor
+        self.c = Fp8MatrixStruct(_ptr(data), _ptr(scales), rows, cols, ld, scale_row_stride, scale_block_stride, type, block_rows)
+        self.addr = C.addressof(self.c)
+        self.rows, self.cols, self.block_rows, self.type = rows, cols, block_rows, type
+        self.tensors = tuple(t for t in (data, scales) if hasattr(t, "is_cuda"))
+
+    @classmethod
+    def of(cls, data, scales, block_rows=1):
+        """From torch tensors: data [rows][cols] of float8_e4m3fn or float8_e5m2 with contiguous columns, scales
+        [ceil(rows / block_rows)][ceil(cols / 128)] of float32 with any strides."""
+        kind = _FP8_TYPES.get(str(data.dtype))
+        if kind is None or str(scales.dtype) != "torch.float32":
+            raise TypeError(f"fp8 matrix of {data.dtype} with scales of {scales.dtype}")
+        rows, cols = data.shape
+        if block_rows not in (1, 128) or tuple(scales.shape) != (-(-rows // block_rows), -(-cols // 128)):
+            raise ValueError(f"scales of shape {tuple(scales.shape)} for {rows} x {cols} codes in blocks of {block_rows} x 128")
+        if cols > 1 and data.stride(1) != 1:
+            raise ValueError("the codes of a row must be contiguous")
+        if rows > 1 and data.stride(0) < cols:
+            raise ValueError("rows of codes overlap")
+        ld = data.stride(0) if rows > 1 else cols
+        if rows == 1 and ld % 16:
+            ld = -(-ld // 16) * 16          # a single row has no pitch: give it one that the copy engine can take
+        return cls(data, scales, rows, cols, ld, scales.stride(0), scales.stride(1), block_rows, kind)
+
+    @classmethod
+    def empty(cls, rows, cols, block_rows=1, type=FP8_E4M3, device="cuda:0"):
+        """Uninitialised, in the layout that the kernels read and write fastest: pitch a multiple of 16 codes; scales of
+        one block column together for block_rows 1, row by row for 128."""
+        import torch
+
+        dt = torch.float8_e4m3fn if type == FP8_E4M3 else torch.float8_e5m2
+        data = torch.empty((rows, -(-cols // 16) * 16), dtype=dt, device=device)[:, :cols]
+        kb = -(-cols // 128)
+        scales = (torch.empty((kb, rows), device=device).t() if block_rows == 1
+                  else torch.empty((-(-rows // block_rows), kb), device=device))
+        return cls.of(data, scales, block_rows)
+
+
 class Context:
     """One decxb context (device, stream, arena).  Pointer arguments are torch tensors, numpy
     arrays or raw integer addresses; leading dimensions are in elements."""
@@ -181,6 +263,7 @@ class Context:
         if rc:
             raise DecxbError(rc, self.L.decxb_status_string(rc).decode())
         self.h = h
+        self.device = device
 
     def close(self):
         if getattr(self, "h", None):
@@ -295,6 +378,58 @@ class Context:
     def release_b(self, pb, stream=None):
         self._chk(self.L.decxb_gemm_release_b(self.h, pb, stream))
 
+    # -- 8-bit linear layer -----------------------------------------------------------------
+    def _here(self, *args):
+        """Tensor arguments have to lie on the context's device (a raw address is the caller's word)."""
+        for a in args:
+            for t in a.tensors if isinstance(a, Fp8Matrix) else (a,):
+                if hasattr(t, "is_cuda") and not (t.is_cuda and t.device.index == self.device):
+                    raise DecxbError(13, f"a tensor on {t.device} was passed to a context of cuda:{self.device}")
+
+    def gemm_fp8(self, A: Fp8Matrix, B: Fp8Matrix, D, ldd, Cin=None, ldc=0, d_type=None, stream=None):
+        """D[A.rows][B.rows] = A B^T (+ Cin), both operands K-contiguous with their block scales (decxb_gemm_fp8)."""
+        self._here(A, B, D, Cin)
+        t = _dtype(D, d_type)
+        if Cin is not None:
+            _dtype(Cin, t)
+        self._chk(self.L.decxb_gemm_fp8(self.h, A.addr, B.addr, _ptr(Cin), ldc, _ptr(D), t, ldd, _stream(stream)))
+
+    def quantize_fp8(self, rows, cols, X, ldx, Q: Fp8Matrix = None, Qt: Fp8Matrix = None, rule=SCALE_AMAX, x_type=None, stream=None):
+        """X [rows][cols] into Q and / or, transposed, into Qt (decxb_quantize_fp8)."""
+        self._here(X, Q, Qt)
+        self._chk(self.L.decxb_quantize_fp8(self.h, _dtype(X, x_type), rows, cols, _ptr(X), ldx, rule,
+                                            Q.addr if Q else None, Qt.addr if Qt else None, _stream(stream)))
+
+    def rmsnorm(self, rows, cols, X, ldx, gamma, eps, R=None, ldr=0, H=None, ldh=0, Y=None, ldy=0, Q: Fp8Matrix = None,
+                rule=SCALE_AMAX, type=None, gamma_type=None, stream=None):
+        """h = X (+ R), y = h / rms(h) * gamma into H, Y and, quantised, Q, whichever are given (decxb_rmsnorm)."""
+        self._here(X, gamma, R, H, Y, Q)
+        t = _dtype(X, type)
+        for a in (R, H, Y):
+            if a is not None:
+                _dtype(a, t)
+        self._chk(self.L.decxb_rmsnorm(self.h, t, rows, cols, _ptr(X), ldx, _ptr(R), ldr, _ptr(gamma), _dtype(gamma, gamma_type),
+                                       eps, _ptr(H), ldh, _ptr(Y), ldy, rule, Q.addr if Q else None, _stream(stream)))
+
+    def rmsnorm_backward_workspace(self, rows, cols) -> int:
+        n = _sz()
+        self._chk(self.L.decxb_rmsnorm_backward_workspace(self.h, rows, cols, C.byref(n)))
+        return n.value
+
+    def rmsnorm_backward(self, rows, cols, dY, lddy, H, ldh, gamma, eps, dX, lddx, dgamma=None, dR=None, lddr=0,
+                         workspace=None, workspace_bytes=0, type=None, gamma_type=None, stream=None):
+        """Gradients of rmsnorm's y: dX (with dR added) and dgamma, fp32 (decxb_rmsnorm_backward)."""
+        self._here(dY, H, gamma, dX, dgamma, dR, workspace)
+        t = _dtype(H, type)
+        for a in (dY, dX, dR):
+            if a is not None:
+                _dtype(a, t)
+        if dgamma is not None:
+            _dtype(dgamma, F32)
+        self._chk(self.L.decxb_rmsnorm_backward(self.h, t, rows, cols, _ptr(dY), lddy, _ptr(H), ldh, _ptr(gamma),
+                                                _dtype(gamma, gamma_type), eps, _ptr(dR), lddr, _ptr(dX), lddx, _ptr(dgamma),
+                                                _ptr(workspace), workspace_bytes, _stream(stream)))
+
     # -- convolution ----------------------------------------------------------------------
     def set_pack_variant(self, variant: int):
         self._chk(self.L.decxb_set_pack_variant(self.h, variant))
@@ -362,6 +497,7 @@ def _order_after_torch(fn):
     def wrapper(self, *args, **kwargs):
         if kwargs.get("stream") is None:
             for a in list(args) + list(kwargs.values()):
+                a = a.data if isinstance(a, Fp8Matrix) else a
                 if getattr(a, "is_cuda", False):
                     import torch
 
@@ -373,7 +509,7 @@ def _order_after_torch(fn):
 
 for _name in ("fill_uniform", "gemm", "gemm_act", "gemm_nt", "gemm_f16", "gemm_batched", "prepare_b", "gemm_prepared",
               "im2col_pack", "conv2_im2col", "conv2_im2col_act", "conv2_im2col_prepared", "conv_prepare_filters",
-              "gemm_rowshard", "conv2_im2col_batchshard"):
+              "gemm_rowshard", "conv2_im2col_batchshard", "gemm_fp8", "quantize_fp8", "rmsnorm", "rmsnorm_backward"):
     setattr(Context, _name, _order_after_torch(getattr(Context, _name)))
 
 

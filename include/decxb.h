@@ -278,6 +278,87 @@ DECXB_API int decxb_gemm_f32_noalloc(int device, int64_t M, int64_t N, int64_t K
                                      const float* C, int64_t ldc, float* D, int64_t ldd,
                                      void* stream, char* err, size_t err_len);
 
+/* ---- 8-bit linear layer ---------------------------------------------------------------
+ * The dense product of a language model's linear layers with operands in 8-bit floating point,
+ * and what feeds it.  No counterpart in the reference, whose narrowest product is the fp16 one.
+ *
+ * An fp8 matrix is rows x cols codes, row-major with cols contiguous, and one fp32 scale for each
+ * block of block_rows x 128 codes (block_rows 1: activations and gradients, 128: weights; the
+ * blocks at the right and bottom edge may be cut).  Element (r, c) stands for
+ *   code(r, c) * scales[(r / block_rows) * scale_row_stride + (c / 128) * scale_block_stride].
+ * The strides are free, so scales may be stored row by row (checkpoints) or block column by block
+ * column; for block_rows 1 scale_row_stride 1 is the layout that the kernels read and write fastest.
+ *
+ * These entries leave the calling thread's current device as it was, are asynchronous on `stream`,
+ * may run at the same time on several streams, and take no scratch memory unless said so at the
+ * entry; calls that take none may be captured into a CUDA graph.  A size of zero rows is a call
+ * without work (DECXB_OK).  Overlap of an output with an input is allowed where the entry says so. */
+typedef enum decxb_dtype { DECXB_F32 = 0, DECXB_F16 = 1, DECXB_BF16 = 2 } decxb_dtype;
+typedef enum decxb_fp8_type {
+    DECXB_FP8_E4M3 = 0,      /* largest value 448, no infinity                    */
+    DECXB_FP8_E5M2 = 1       /* largest finite value 57344                        */
+} decxb_fp8_type;
+typedef enum decxb_scale_rule {
+    DECXB_SCALE_AMAX = 0,    /* scale = max|x| of the block / largest value of the type  */
+    DECXB_SCALE_POW2 = 1     /* the same rounded up to a power of two                     */
+} decxb_scale_rule;
+typedef struct decxb_fp8_matrix {
+    void*   data;                 /* rows x cols codes                                     */
+    float*  scales;
+    int64_t rows, cols, ld;       /* ld: codes from one row to the next, >= cols           */
+    int64_t scale_row_stride;     /* scales from one row of blocks to the next, >= 0       */
+    int64_t scale_block_stride;   /* scales from one block of a row to the next, >= 0      */
+    int32_t type;                 /* decxb_fp8_type                                        */
+    int32_t block_rows;           /* 1 or 128                                              */
+} decxb_fp8_matrix;
+
+/* D[M][N] = sum over k of A[m][k] * B[n][k] (+ C[m][n]) with M = A->rows, N = B->rows and
+ * K = A->cols = B->cols >= 1: both operands K-contiguous, as a linear layer keeps x [tokens][in] and
+ * its weight [out][in].  The products of one block of 128 are summed by the tensor cores
+ * (tcgen05 kind::f8f6f4, fp32), scaled by both blocks' scales and added in IEEE fp32; D and C are
+ * of d_type and rounded once.  A and B may be of different fp8 types; either may have block_rows
+ * 1 or 128.  C may be D itself (same pointer and leading dimension); otherwise D overlaps nothing.
+ * Data whose address or ld is not a multiple of 16 bytes is first copied into arena scratch
+ * (such a call cannot be captured: DECXB_ERR_BAD_PARAM); other calls take no scratch.
+ * The product of two scales should be a finite fp32 number. */
+DECXB_API int decxb_gemm_fp8(decxb_ctx* ctx, const decxb_fp8_matrix* A, const decxb_fp8_matrix* B,
+                             const void* C, int64_t ldc, void* D, int d_type, int64_t ldd, void* stream);
+
+/* Quantises X [rows][cols] of x_type: Q (rows x cols) and Qt (cols x rows, the transpose, its blocks
+ * running along X's rows) where given, at least one of the two.  Per block: scale by `scale_rule`,
+ * at least 2^-126 (a block of zeros has that scale and zero codes); code = x * (1 / scale) rounded to
+ * nearest even.  A block that holds a NaN has scale and codes NaN; one that holds an infinity has
+ * scale infinity, its finite values give 0 and its infinities NaN.  cols may be 0 or rows may be 0:
+ * nothing is written.  Bytes of Q between cols and ld are left as they were. */
+DECXB_API int decxb_quantize_fp8(decxb_ctx* ctx, int x_type, int64_t rows, int64_t cols, const void* X, int64_t ldx,
+                                 int scale_rule, const decxb_fp8_matrix* Q, const decxb_fp8_matrix* Qt, void* stream);
+
+/* Root-mean-square norm with the residual's addition, row by row:
+ *   h = X + R (R may be NULL: h = X),  y = h / sqrt(mean(h^2) + eps) * gamma.
+ * Writes what is given of H (h, rounded to `type`), Y (y, rounded to `type`) and Q (y quantised as
+ * decxb_quantize_fp8 does, block_rows 1); at least one of the three.  X, R, H, Y are [rows][cols] of
+ * `type`, gamma is cols values of gamma_type; statistics, h and y are fp32 until they are rounded.
+ * H or Y may be X or R itself (same pointer and leading dimension), H and Y are different. */
+DECXB_API int decxb_rmsnorm(decxb_ctx* ctx, int type, int64_t rows, int64_t cols, const void* X, int64_t ldx,
+                            const void* R, int64_t ldr, const void* gamma, int gamma_type, float eps,
+                            void* H, int64_t ldh, void* Y, int64_t ldy,
+                            int scale_rule, const decxb_fp8_matrix* Q, void* stream);
+
+/* Gradient of y = h / sqrt(mean(h^2) + eps) * gamma, row by row, with r = 1 / sqrt(mean(h^2) + eps):
+ *   dX = dR + r * (dY * gamma - h * r^2 * mean(dY * gamma * h)),   dgamma = sum over rows of dY * h * r.
+ * dY, H, dR, dX are [rows][cols] of `type`; dR (NULL: 0) is the gradient that reaches h directly, through
+ * the residual path, and dX is the gradient of both X and R of the forward entry.  dgamma is cols
+ * fp32 values, overwritten (zeros for rows = 0); NULL: not computed.  dX may be dY or dR itself.  The sum over
+ * rows is taken in an order that the sizes alone fix.  It needs decxb_rmsnorm_backward_workspace bytes
+ * (0 without dgamma), 16-byte aligned, that no other call uses at the same time; workspace NULL
+ * takes them from the arena in stream order, which cannot be captured (DECXB_ERR_BAD_PARAM). */
+DECXB_API int decxb_rmsnorm_backward_workspace(decxb_ctx* ctx, int64_t rows, int64_t cols, size_t* bytes);
+DECXB_API int decxb_rmsnorm_backward(decxb_ctx* ctx, int type, int64_t rows, int64_t cols,
+                                     const void* dY, int64_t lddy, const void* H, int64_t ldh,
+                                     const void* gamma, int gamma_type, float eps,
+                                     const void* dR, int64_t lddr, void* dX, int64_t lddx, float* dgamma,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- im2col convolution --------------------------------------------------------------
  * Geometry shared by the entry points below (conv2_mk_im2col.h:60-93, :170-199). */
 typedef struct decxb_conv_geom {
