@@ -55,6 +55,7 @@ struct Params {
     void* D; int64_t ldd;
     int d_type;
     bool tma_store;                /* D leaves through the copy engine                 */
+    bool d_vec;                    /* four results of a row may leave in one store      */
     long long wait_limit_ns;
     decxb_dev_status* status;
 };
@@ -139,6 +140,18 @@ __device__ __forceinline__ float lds_f32(uint32_t at)
     float v; asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory"); return v;
 }
 
+__device__ __forceinline__ float2 lds_f32x2(uint32_t at)
+{
+    float2 v; asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory"); return v;
+}
+/* From the shared memory of a CTA of the cluster. */
+__device__ __forceinline__ float4 lds_cluster_f32x4(uint32_t at)
+{
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+
 __device__ __forceinline__ float4 lds_f32x4(uint32_t at)
 {
     float4 v; asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory"); return v;
@@ -199,14 +212,38 @@ __device__ __forceinline__ void box_rows(const Params& p, uint32_t box, int lane
     }
 }
 
+/* Up to four adjacent results: (+C), one rounding, one store where the rows allow it. */
+template <typename T>
+__device__ __forceinline__ void put4(const Params& p, int64_t row, int64_t col, int have, float4 v)
+{
+    T* d = static_cast<T*>(p.D) + row * p.ldd + col;
+    float f[4] = {v.x, v.y, v.z, v.w};
+    if (p.C) {
+        const T* c = static_cast<const T*>(p.C) + row * p.ldc + col;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) if (j < have) f[j] += to_f32(c[j]);
+    }
+    if (have == 4 && p.d_vec) {
+        alignas(16) T o[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = from_f32<T>(f[j]);
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(d) = *reinterpret_cast<const uint4*>(o);
+        else                          *reinterpret_cast<uint2*>(d) = *reinterpret_cast<const uint2*>(o);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) if (j < have) d[j] = from_f32<T>(f[j]);
+    }
+}
+
 /* --------------------------------------------------------------------------------------
- * CTAS   : 1 or 2 CTAs per tile (cta_group)
- * BN     : rows of B loaded per CTA; the tile is 128 CTAS x BN CTAS
+ * Many result tiles: a pair of CTAs (cta_group::2) per tile of 256 x 256, each with 128 rows of A and 128 of B.
  * COLVEC : B has a scale per row (block_rows 1): each column of the tile has its own factor.  Otherwise a
  *          128-row block of B has one scale, and the columns of one epilogue warp lie in one block.
  * ------------------------------------------------------------------------------------ */
-template <int CTAS, int BN, bool COLVEC>
+template <bool COLVEC>
 struct Cfg {
+    static constexpr int CTAS = 2;
+    static constexpr int BN = 128;                             /* rows of B per CTA */
     static constexpr int UMMA_M = BM_CTA * CTAS;
     static constexpr int UMMA_N = BN * CTAS;
     static constexpr int ACC = UMMA_N / 2;                     /* columns per epilogue warp */
@@ -216,26 +253,21 @@ struct Cfg {
     static constexpr int KB_FLOATS = BM_CTA + (COLVEC ? UMMA_N : 32);
     static constexpr int SCALE_BYTES = SLOTS * KB_FLOATS * 4;
     static constexpr int BOX_BYTES = EPI_WARPS * 4096;         /* result boxes, one a warp */
-    static constexpr int STAGES_RAW = (SMEM_LIMIT - 2048 - SCALE_BYTES - BOX_BYTES) / STAGE_BYTES;
-    static constexpr int STAGES = STAGES_RAW > 8 ? 8 : STAGES_RAW;
+    static constexpr int STAGES = (SMEM_LIMIT - 2048 - SCALE_BYTES - BOX_BYTES) / STAGE_BYTES;
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + BOX_BYTES + SCALE_BYTES + 1024 /* alignment slack */ + 512 /* barriers */;
-    static constexpr int BUFS = 512 / UMMA_N > 4 ? 4 : 512 / UMMA_N;      /* accumulators in tensor memory */
+    static constexpr int BUFS = 512 / UMMA_N;                  /* accumulators in tensor memory */
     static constexpr int TMEM_COLS = BUFS * UMMA_N;
-    /* 128 running sums per thread need the registers of warp group 0: see the launch */
-    static constexpr bool REALLOC = ACC > 64;
-    static_assert(UMMA_N % 64 == 0 && UMMA_N <= 256 && ACC <= 128, "tile width");
     static_assert(SMEM_BYTES <= SMEM_LIMIT, "shared memory");
-    static_assert(BUFS == 2 || BUFS == 4, "buffers alternate between two issuers");
-    /* the epilogue reads a stage's barrier by parity and lies at most BUFS k-blocks behind the issuers */
+    /* the epilogue reads a stage's barrier by parity and lies at most BUFS k-blocks behind the issuer */
     static_assert(STAGES > BUFS, "a stage's barrier must not turn over twice unseen");
 };
 
-template <int CTAS, int BN, bool COLVEC>
+template <bool COLVEC>
 __global__ void __launch_bounds__(THREADS, 1)
 decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                       const __grid_constant__ CUtensorMap map_d, const Params p)
 {
-    using C = Cfg<CTAS, BN, COLVEC>;
+    using C = Cfg<COLVEC>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;     /* the swizzle is a function of address bits 4-9 */
     const uint32_t boxes = smem_base + C::STAGES * C::STAGE_BYTES;
@@ -251,34 +283,37 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     auto stage_b = [&](int s) { return smem_base + s * C::STAGE_BYTES + C::A_BYTES; };
 
     const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const uint32_t cta_rank = CTAS == 2 ? cluster_ctarank() : 0u;
+    const uint32_t cta_rank = cluster_ctarank();
     const bool is_leader = cta_rank == 0;
-    const int cluster_id = (int)blockIdx.x / CTAS, num_clusters = (int)gridDim.x / CTAS;
+    const int cluster_id = (int)blockIdx.x / C::CTAS, num_clusters = (int)gridDim.x / C::CTAS;
     const int num_tiles = p.tiles_m * p.tiles_n;
 
     if (threadIdx.x == 0) {
         prefetch_tensormap(&map_a); prefetch_tensormap(&map_b);
         if (p.tma_store) prefetch_tensormap(&map_d);
         for (int s = 0; s < C::STAGES; ++s) { mbar_init(full_bar(s), 1); mbar_init(done_bar(s), 1); }
-        for (int b = 0; b < C::BUFS; ++b) mbar_init(tempty_bar(b), EPI_WARPS * CTAS);
+        for (int b = 0; b < C::BUFS; ++b) mbar_init(tempty_bar(b), EPI_WARPS * C::CTAS);
         for (int s = 0; s < SLOTS; ++s) { mbar_init(sfull_bar(s), 32); mbar_init(sempty_bar(s), EPI_WARPS); }
         fence_barrier_init();
     }
     if (warp == 1) {
-        tmem_alloc<CTAS>(tmem_slot, C::TMEM_COLS);
-        tmem_relinquish<CTAS>();
+        tmem_alloc<C::CTAS>(tmem_slot, C::TMEM_COLS);
+        tmem_relinquish<C::CTAS>();
     }
     tc_fence_before();
     __syncthreads();
-    if (CTAS == 2) cluster_sync_all();
+    cluster_sync_all();
     tc_fence_after();
     uint32_t tmem_base;
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot));
+    /* the next kernel of the stream may take this one's place as its blocks leave; this one starts on the memory of
+     * the kernels before it only when they have completed */
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
     if (warp < 4) {
         /* 168 registers a thread at launch: 128 * 56 + 256 * 224 = 64512 = 384 * 168 */
-        if constexpr (C::REALLOC) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 0) {
             /* -------------------------------------------------------- TMA producer ---- */
             int stage = 0; uint32_t phase = 0;
@@ -287,22 +322,15 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
             for (int t = cluster_id; t < num_tiles && alive; t += num_clusters) {
                 int tm, tn; tile_coords(t, p.tiles_m, p.tiles_n, p.tile_group, tm, tn);
                 const int row_a = tm * C::UMMA_M + (int)cta_rank * BM_CTA;
-                const int row_b = tn * C::UMMA_N + (int)cta_rank * BN;
+                const int row_b = tn * C::UMMA_N + (int)cta_rank * C::BN;
                 for (int kb = 0; kb < p.num_kb; ++kb) {
                     if (!warp_wait(done_bar(stage), phase ^ 1u, p, 1100 + stage, t)) { alive = false; break; }
                     if (elect_one()) {
-                        if (CTAS == 1) {
-                            const uint32_t fb = full_bar(stage);
-                            mbar_arrive_expect_tx(fb, C::STAGE_BYTES);
-                            tma_load_2d(stage_a(stage), &map_a, fb, kb * BK, row_a);
-                            tma_load_2d(stage_b(stage), &map_b, fb, kb * BK, row_b);
-                        } else {
-                            /* both CTAs' bytes are counted on the leader's barrier */
-                            if (is_leader) mbar_arrive_expect_tx(full_bar(stage), 2 * C::STAGE_BYTES);
-                            const uint32_t fb = mapa(full_bar(stage), 0);
-                            tma_load_2d_pair(stage_a(stage), &map_a, fb, kb * BK, row_a);
-                            tma_load_2d_pair(stage_b(stage), &map_b, fb, kb * BK, row_b);
-                        }
+                        /* both CTAs' bytes are counted on the leader's barrier */
+                        if (is_leader) mbar_arrive_expect_tx(full_bar(stage), 2 * C::STAGE_BYTES);
+                        const uint32_t fb = mapa(full_bar(stage), 0);
+                        tma_load_2d_pair(stage_a(stage), &map_a, fb, kb * BK, row_a);
+                        tma_load_2d_pair(stage_b(stage), &map_b, fb, kb * BK, row_b);
                     }
                     __syncwarp();
                     armed |= 1u << stage;
@@ -337,9 +365,9 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
 #pragma unroll
                             for (int kk = 0; kk < BK / UMMA_K; ++kk) {
                                 const uint64_t koff = (uint64_t)((kk * UMMA_K) >> 4);
-                                umma_fp8<CTAS>(tmem_d, da + koff, db + koff, p.idesc, kk != 0 ? 1u : 0u);
+                                umma_fp8<C::CTAS>(tmem_d, da + koff, db + koff, p.idesc, kk != 0 ? 1u : 0u);
                             }
-                            umma_commit<CTAS>(done_bar(stage));
+                            umma_commit<C::CTAS>(done_bar(stage));
                         }
                         __syncwarp();
                         if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
@@ -381,7 +409,7 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         }
     } else {
         /* ------------------------------------------------------------ epilogue -------- */
-        if constexpr (C::REALLOC) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int q = warp & 3, eh = (warp - 4) >> 2;
         const uint32_t tlane = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(eh * C::ACC);
         const uint32_t box = boxes + (uint32_t)(warp - 4) * 4096u;
@@ -426,8 +454,8 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                 tc_fence_before();
                 __syncwarp();
                 if (elect_one()) {
-                    if (CTAS == 1 || is_leader) mbar_arrive(tempty_bar(acc));
-                    else                        mbar_arrive_leader(tempty_bar(acc));
+                    if (is_leader) mbar_arrive(tempty_bar(acc));
+                    else           mbar_arrive_leader(tempty_bar(acc));
                     mbar_arrive(sempty_bar(slot));
                 }
                 __syncwarp();
@@ -476,10 +504,266 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     /* ---------------------------------------------------------------- teardown -------- */
     tc_fence_before();
     __syncthreads();
-    if (CTAS == 2) cluster_sync_all();
+    cluster_sync_all();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc<CTAS>(tmem_base, C::TMEM_COLS);
+        tmem_dealloc<C::CTAS>(tmem_base, C::TMEM_COLS);
+    }
+}
+
+/* --------------------------------------------------------------------------------------
+ * Few result tiles: the same product with the roles of the operands exchanged and K split over a cluster.
+ *
+ * A tile is 128 rows of B (the accumulator's lanes) by NT rows of A (its columns, 16 to 128 tokens), so one token
+ * pads the tensor core's tile to 16 columns instead of 128 rows; the CTAs of a cluster take a share of the
+ * k-blocks each, and their fp32 sums meet through distributed shared memory: no workspace, no atomics, one order.
+ * Bound by the weights' bytes for few tokens (a k-block brings 16 KiB of B whatever NT is).
+ * Tensor memory is read in the shape in which a thread holds two adjacent columns of every eight for four rows
+ * (16x256b), so that a warp's column factors come in a quarter of the shared-memory reads of one row a thread.
+ * ------------------------------------------------------------------------------------ */
+template <int NT>
+struct SplitCfg {
+    static constexpr int CTAS_PER_SM = NT == 128 ? 1 : 2;      /* at most, when the launch asks for half of the shared memory */
+    static constexpr int CW = NT / 2;                          /* columns per epilogue warp */
+    static constexpr int W_BYTES = BM_CTA * BK;
+    static constexpr int STAGE_BYTES = W_BYTES + NT * BK;
+    static constexpr int KB_FLOATS = BM_CTA + NT;
+    static constexpr int SCALE_BYTES = SLOTS * KB_FLOATS * 4;
+    static constexpr int PITCH = BM_CTA + 4;                   /* of the partial sums [NT][PITCH]: no bank twice in a store */
+    static constexpr int OTHER_BYTES = SCALE_BYTES + 1024 /* alignment slack */ + 512 /* barriers */;
+    static constexpr int MOST_STAGES = 12;
+    /* stages of a launch with one or two CTAs per SM */
+    static constexpr int stages(int ctas_per_sm)
+    {
+        const int n = ((ctas_per_sm == 2 ? 113 * 1024 : SMEM_LIMIT) - OTHER_BYTES) / STAGE_BYTES;
+        return n > MOST_STAGES ? MOST_STAGES : n;
+    }
+    static constexpr int BUFS = stages(CTAS_PER_SM) > 4 ? 4 : stages(CTAS_PER_SM) - 1;   /* fewer than stages: their barriers are read by parity */
+    static constexpr int TMEM_COLS = 4 * NT;
+    static_assert(BUFS >= 2, "buffers");
+    static_assert(NT * PITCH * 4 <= stages(CTAS_PER_SM) * STAGE_BYTES, "partial sums reuse the stages");
+};
+
+/* 16 lanes x 8 G columns: register 4 g + k is column 8 g + 2 (lane % 4) + (k & 1) of lane lane / 4 + 8 (k >> 1). */
+template <int G>
+__device__ __forceinline__ void tmem_ld_16x256(uint32_t taddr, float* v)
+{
+    if constexpr (G == 1)
+        asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(taddr) : "memory");
+    else if constexpr (G == 2)
+        asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "r"(taddr) : "memory");
+    else
+        asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
+                       "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]) : "r"(taddr) : "memory");
+}
+/* tcgen05.wait::ld with n loaded registers as operands (see tmem_ld_wait32). */
+template <int N>
+__device__ __forceinline__ void tmem_ld_wait_n(float* v)
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]) :: "memory");
+#pragma unroll
+    for (int i = 4; i < N; ++i) asm volatile("" : "+f"(v[i]) :: "memory");
+}
+
+template <int NT>
+__global__ void __launch_bounds__(THREADS, SplitCfg<NT>::CTAS_PER_SM)
+decxb_gemm_fp8_split_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const Params p, const int splits, const int stages)
+{
+    using C = SplitCfg<NT>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t ring = smem_base + stages * C::STAGE_BYTES;
+    const uint32_t bars = ring + C::SCALE_BYTES;
+    auto full_bar   = [&](int s) { return bars + 8u * s; };
+    auto done_bar   = [&](int s) { return bars + 8u * (C::MOST_STAGES + s); };
+    auto tempty_bar = [&](int b) { return bars + 8u * (2 * C::MOST_STAGES + b); };
+    auto sfull_bar  = [&](int s) { return bars + 8u * (2 * C::MOST_STAGES + C::BUFS + s); };
+    auto sempty_bar = [&](int s) { return bars + 8u * (2 * C::MOST_STAGES + C::BUFS + SLOTS + s); };
+    const uint32_t tmem_slot = bars + 8u * (2 * C::MOST_STAGES + C::BUFS + 2 * SLOTS);
+    auto stage_w = [&](int s) { return smem_base + s * C::STAGE_BYTES; };
+    auto stage_x = [&](int s) { return smem_base + s * C::STAGE_BYTES + C::W_BYTES; };
+
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const int tile = (int)blockIdx.x / splits, rank = (int)blockIdx.x % splits;
+    const int tn = tile / p.tiles_m, tm = tile - tn * p.tiles_m;            /* tokens fastest: their tiles share the weights in L2 */
+    const int n0 = tn * BM_CTA, m0 = tm * NT;
+    const int kb_first = (int)((int64_t)p.num_kb * rank / splits), kb_last = (int)((int64_t)p.num_kb * (rank + 1) / splits);
+
+    if (threadIdx.x == 0) {
+        prefetch_tensormap(&map_w); prefetch_tensormap(&map_x);
+        for (int s = 0; s < stages; ++s) { mbar_init(full_bar(s), 1); mbar_init(done_bar(s), 1); }
+        for (int b = 0; b < C::BUFS; ++b) mbar_init(tempty_bar(b), EPI_WARPS);
+        for (int s = 0; s < SLOTS; ++s) { mbar_init(sfull_bar(s), 32); mbar_init(sempty_bar(s), EPI_WARPS); }
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        tmem_alloc<1>(tmem_slot, C::TMEM_COLS);
+        tmem_relinquish<1>();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    uint32_t tmem_base;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem_base) : "r"(tmem_slot));
+    /* the next kernel of the stream may take this one's place as its blocks leave; this one starts on the memory of
+     * the kernels before it only when they have completed */
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    if (warp == 0) {
+        /* ------------------------------------------------------------ TMA producer ---- */
+        int stage = 0; uint32_t phase = 0;
+        uint32_t armed = 0, armed_parity = 0;
+        for (int kb = kb_first; kb < kb_last; ++kb) {
+            if (!warp_wait(done_bar(stage), phase ^ 1u, p, 2100 + stage, tile)) break;
+            if (elect_one()) {
+                const uint32_t fb = full_bar(stage);
+                mbar_arrive_expect_tx(fb, C::STAGE_BYTES);
+                tma_load_2d(stage_w(stage), &map_w, fb, kb * BK, n0);
+                tma_load_2d(stage_x(stage), &map_x, fb, kb * BK, m0);
+            }
+            __syncwarp();
+            armed |= 1u << stage;
+            armed_parity = (armed_parity & ~(1u << stage)) | (phase << stage);
+            if (++stage == stages) { stage = 0; phase ^= 1u; }
+        }
+        if (lane == 0 && *reinterpret_cast<volatile int*>(&p.status->code) != 0) {       /* copies still on their way */
+            for (int s2 = 0; s2 < stages; ++s2) {
+                if (!((armed >> s2) & 1u)) continue;
+                for (int tries = 0; tries < 2048 && !mbar_try_wait(full_bar(s2), (armed_parity >> s2) & 1u); ++tries) __nanosleep(64);
+            }
+        }
+    } else if (warp == 1) {
+        /* ------------------------------------------------------------ MMA issuer ------ */
+        int stage = 0; uint32_t phase = 0;
+        for (int unit = 0; unit < kb_last - kb_first; ++unit) {
+            const int acc = unit % C::BUFS;
+            if (!warp_wait(full_bar(stage), phase, p, 2300 + stage, tile)) break;
+            if (!warp_wait(tempty_bar(acc), ((uint32_t)(unit / C::BUFS) & 1u) ^ 1u, p, 2200 + acc, tile)) break;
+            tc_fence_after();
+            if (elect_one()) {
+                const uint32_t tmem_d = tmem_base + (uint32_t)(acc * NT);
+                const uint64_t dw = make_smem_desc(stage_w(stage)), dx = make_smem_desc(stage_x(stage));
+#pragma unroll
+                for (int kk = 0; kk < BK / UMMA_K; ++kk) {
+                    const uint64_t koff = (uint64_t)((kk * UMMA_K) >> 4);
+                    umma_fp8<1>(tmem_d, dw + koff, dx + koff, p.idesc, kk != 0 ? 1u : 0u);
+                }
+                umma_commit<1>(done_bar(stage));
+            }
+            __syncwarp();
+            if (++stage == stages) { stage = 0; phase ^= 1u; }
+        }
+    } else if (warp == 2) {
+        /* ------------------------------------------------------------ scale loader ---- */
+        constexpr int NX = (NT + 31) / 32;
+        const float* src[4 + NX];
+        uint32_t exists = 0;
+#pragma unroll
+        for (int i = 0; i < 4 + NX; ++i) {
+            const bool w = i < 4;
+            const int at = (w ? i : i - 4) * 32 + lane;
+            int64_t r = (int64_t)(w ? n0 : m0) + at;
+            if (r < (w ? p.N : p.M) && (w || at < NT)) exists |= 1u << i; else r = 0;
+            src[i] = w ? p.sb.p + (r >> p.sb.shift) * p.sb.rs + kb_first * p.sb.ks : p.sa.p + (r >> p.sa.shift) * p.sa.rs + kb_first * p.sa.ks;
+        }
+        int slot = 0; uint32_t phase = 0;
+        for (int kb = kb_first; kb < kb_last; ++kb) {
+            if (!warp_wait(sempty_bar(slot), phase ^ 1u, p, 2500 + slot, tile)) break;
+            const uint32_t dst = ring + (uint32_t)(slot * C::KB_FLOATS + lane) * 4u;
+#pragma unroll
+            for (int i = 0; i < 4 + NX; ++i) {
+                if (i < 4 || NT >= 32 || lane < NT) cp_async4(dst + i * 128u, src[i], (exists >> i) & 1u);
+                src[i] += i < 4 ? p.sb.ks : p.sa.ks;
+            }
+            cp_async_arrive(sfull_bar(slot));
+            if (++slot == SLOTS) { slot = 0; phase ^= 1u; }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else if (warp >= 4) {
+        /* ------------------------------------------------------------ sums ------------ */
+        const int q = warp & 3, eh = (warp - 4) >> 2;
+        constexpr int G = C::CW >= 32 ? 4 : C::CW / 8;         /* groups of eight columns per load */
+        const uint32_t tlane = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(eh * C::CW);
+        float sum[C::CW];                                      /* [columns / 8 G][lane half][G][4] */
+#pragma unroll
+        for (int i = 0; i < C::CW; ++i) sum[i] = 0.0f;
+        int stage = 0, slot = 0;
+        uint32_t phase = 0, sphase = 0;
+        for (int unit = 0; unit < kb_last - kb_first; ++unit) {
+            const int acc = unit % C::BUFS;
+            if (!warp_wait(sfull_bar(slot), sphase, p, 2600 + slot, tile)) break;
+            const uint32_t sc = ring + (uint32_t)(slot * C::KB_FLOATS) * 4u;
+            float sw[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sw[i] = lds_f32(sc + (uint32_t)(q * 32 + i * 8 + (lane >> 2)) * 4u);
+            if (!warp_wait(done_bar(stage), phase, p, 2400 + stage, tile)) break;
+            tc_fence_after();
+#pragma unroll
+            for (int c = 0; c < C::CW; c += 8 * G) {
+                float v[8 * G];
+                tmem_ld_16x256<G>(tlane + (uint32_t)(acc * NT + c), v);
+                tmem_ld_16x256<G>(tlane + (16u << 16) + (uint32_t)(acc * NT + c), v + 4 * G);
+                tmem_ld_wait_n<8 * G>(v);
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    const float2 x = lds_f32x2(sc + (uint32_t)(BM_CTA + eh * C::CW + c + g * 8 + (lane & 3) * 2) * 4u);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const int i = h * 4 * G + g * 4 + k;
+                            sum[c + i] = fmaf(v[i], sw[2 * h + (k >> 1)] * ((k & 1) ? x.y : x.x), sum[c + i]);
+                        }
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (elect_one()) { mbar_arrive(tempty_bar(acc)); mbar_arrive(sempty_bar(slot)); }
+            __syncwarp();
+            if (++slot == SLOTS) { slot = 0; sphase ^= 1u; }
+            if (++stage == stages) { stage = 0; phase ^= 1u; }
+        }
+        /* every MMA of this CTA has run, so the stages can hold its sums: [token][row of B] */
+#pragma unroll
+        for (int c = 0; c < C::CW; c += 8 * G)
+#pragma unroll
+            for (int i = 0; i < 8 * G; ++i) {
+                const int h = i / (4 * G), g = (i / 4) % G, k = i & 3;
+                const int m = eh * C::CW + c + g * 8 + (lane & 3) * 2 + (k & 1), n = q * 32 + h * 16 + (k >> 1) * 8 + (lane >> 2);
+                asm volatile("st.shared.f32 [%0], %1;" :: "r"(smem_base + (uint32_t)(m * C::PITCH + n) * 4u), "f"(sum[c + i]) : "memory");
+            }
+    }
+    __syncwarp();
+    tc_fence_before();
+    if (splits > 1) cluster_sync_all(); else __syncthreads();
+
+    /* each CTA finishes its share of the tokens, eight at a time, four columns a thread: the cluster's sums in ascending
+     * order, addend, one rounding */
+    if (warp >= 4) {
+        const int t = (int)threadIdx.x - 128, n = n0 + (t & 31) * 4, rows = (int)min((int64_t)NT, p.M - m0);
+        const int have = (int)min((int64_t)4, p.N - n);
+        for (int m = rank * 8 + (t >> 5); m < rows && have > 0; m += 8 * splits) {
+            const uint32_t at = smem_base + (uint32_t)(m * C::PITCH + (t & 31) * 4) * 4u;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+            for (int r = 0; r < splits; ++r) {
+                const float4 w = splits > 1 ? lds_cluster_f32x4(mapa(at, (uint32_t)r)) : lds_f32x4(at);
+                v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+            }
+            if (p.d_type == DECXB_F32)      put4<float>(p, m0 + m, n, have, v);
+            else if (p.d_type == DECXB_F16) put4<__half>(p, m0 + m, n, have, v);
+            else                            put4<__nv_bfloat16>(p, m0 + m, n, have, v);
+        }
+    }
+    __syncwarp();
+    if (splits > 1) cluster_sync_all(); else __syncthreads();      /* the peers have read this CTA's sums */
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc<1>(tmem_base, C::TMEM_COLS);
     }
 }
 
@@ -506,11 +790,11 @@ int make_map_fp8(decxb_ctx* ctx, CUtensorMap* map, const decxb_fp8_matrix& m, in
     return make_map_2d(ctx, map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, m.data, m.rows, m.cols, m.ld, box_rows);
 }
 
-template <int CTAS, int BN, bool COLVEC>
+template <bool COLVEC>
 int launch(decxb_ctx* ctx, const decxb_fp8_matrix& A, const decxb_fp8_matrix& B, Params p, cudaStream_t s)
 {
-    using C = Cfg<CTAS, BN, COLVEC>;
-    auto kernel = decxb_gemm_fp8_kernel<CTAS, BN, COLVEC>;
+    using C = Cfg<COLVEC>;
+    auto kernel = decxb_gemm_fp8_kernel<COLVEC>;
     static std::once_flag once[DECXB_MAX_DEVICES];
     static cudaError_t attr_err[DECXB_MAX_DEVICES];
     static int regs[DECXB_MAX_DEVICES];
@@ -523,10 +807,10 @@ int launch(decxb_ctx* ctx, const decxb_fp8_matrix& A, const decxb_fp8_matrix& B,
     });
     if (attr_err[dev] != cudaSuccess) return decxb_fail(ctx, DECXB_ERR_CUDA, std::string("fp8 kernel attributes: ") + cudaGetErrorString(attr_err[dev]));
     /* a register hand-over that does not add up would wait forever: never launch it */
-    if (C::REALLOC && regs[dev] != 168) return decxb_fail(ctx, DECXB_ERR_CUDA, "fp8 GEMM kernel was not compiled to 168 registers");
+    if (regs[dev] != 168) return decxb_fail(ctx, DECXB_ERR_CUDA, "fp8 GEMM kernel was not compiled to 168 registers");
     CUtensorMap ma, mb;
     int rc;
-    if ((rc = make_map_fp8(ctx, &ma, A, BM_CTA)) || (rc = make_map_fp8(ctx, &mb, B, BN))) return rc;
+    if ((rc = make_map_fp8(ctx, &ma, A, BM_CTA)) || (rc = make_map_fp8(ctx, &mb, B, C::BN))) return rc;
     CUtensorMap md = ma;
     if (p.tma_store) {
         const int e = size_of(p.d_type);
@@ -538,21 +822,136 @@ int launch(decxb_ctx* ctx, const decxb_fp8_matrix& A, const decxb_fp8_matrix& B,
     if (tm * tn > 0x7fffffffLL) return decxb_fail(ctx, DECXB_ERR_TOO_LARGE, "fp8 gemm tiles");
     p.tiles_m = (int)tm; p.tiles_n = (int)tn;
     p.idesc = make_idesc_fp8(C::UMMA_M, C::UMMA_N, A.type, B.type);
-    int64_t clusters = (ctx->sm_count - ctx->reserved_sms) / CTAS;
+    int64_t clusters = (ctx->sm_count - ctx->reserved_sms) / C::CTAS;
     if (clusters > tm * tn) clusters = tm * tn;
     if (clusters < 1) clusters = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(clusters * CTAS), 1, 1);
+    cfg.gridDim = dim3((unsigned)(clusters * C::CTAS), 1, 1);
     cfg.blockDim = dim3(THREADS, 1, 1);
     cfg.dynamicSmemBytes = C::SMEM_BYTES;
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = CTAS; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr; cfg.numAttrs = 1;
+    attr[0].val.clusterDim.x = C::CTAS; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
     decxb_launch_scope scope(ctx, s, DECXB_K_GEMM);
     DECXB_CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, kernel, ma, mb, md, p));
     return DECXB_OK;
+}
+
+/* The launch of a split product but for its stream: `clusters` clusters of `splits` CTAs, `per_sm` CTAs to an SM. */
+template <int NT>
+cudaLaunchConfig_t split_config(cudaLaunchAttribute* attr, int64_t clusters, int splits, int per_sm)
+{
+    using C = SplitCfg<NT>;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(clusters * splits), 1, 1);
+    cfg.blockDim = dim3(THREADS, 1, 1);
+    cfg.dynamicSmemBytes = (size_t)C::stages(per_sm) * C::STAGE_BYTES + C::OTHER_BYTES;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)splits; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = 2;
+    return cfg;
+}
+
+/* How many clusters of 1, 2, 4 and 8 CTAs the device holds at once with one CTA to an SM (asked once): the SMs of a cluster lie
+ * in one group of SMs, so it is less than the SMs divided by the size. */
+struct Resident { int clusters[4]; cudaError_t err; };
+
+template <int NT>
+const Resident& resident(decxb_ctx* ctx)
+{
+    static std::once_flag once[DECXB_MAX_DEVICES];
+    static Resident table[DECXB_MAX_DEVICES];
+    Resident& t = table[ctx->device];
+    std::call_once(once[ctx->device], [&] {
+        auto kernel = decxb_gemm_fp8_split_kernel<NT>;
+        t.err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_LIMIT);
+        for (int i = 0; i < 4 && t.err == cudaSuccess; ++i) {
+            cudaLaunchAttribute attr[2];
+            cudaLaunchConfig_t cfg = split_config<NT>(attr, 1, 1 << i, 1);
+            cfg.numAttrs = 1;
+            t.err = cudaOccupancyMaxActiveClusters(&t.clusters[i], kernel, &cfg);
+        }
+    });
+    return t;
+}
+
+/* How a product is cut: `splits` shares of K, `per_sm` CTAs to an SM (two have half the stages each), and what it takes, in
+ * microseconds (fitted to 65 <= M <= 1024, 1024 <= N <= 32768, 1024 <= K <= 16384 on a B200).
+ *  - The largest power of two of shares of which one wave of clusters holds all (2048 columns, K = 4096, one token: 2, 4, 8
+ *    shares 6.6, 4.7, 8.2 us, eight being two waves), but no share below four k-blocks (1 x 4096 x 1024: two shares
+ *    3.9, four 4.3, eight 5.2 us).
+ *  - Up to 64 tokens, where that leaves a fifth of the SMs empty, twice the shares with two CTAs to an SM (1 x 12000 x 4096:
+ *    11.4 and 10.3 us; 1 x 6000 x 4096: 7.3 and 6.9), though not eight (33 x 2048 x 4096, four and eight: 6.4 and 7.1).
+ *    Two CTAs to an SM as well where there are more tiles than SMs (64 x 32768 x 4096: 32.3 and 26.4). Otherwise one CTA
+ *    with all of the shared memory has the longer queue of loads (48 x 4096 x 8192: 10.3 and 14.6). */
+struct Cut { int splits, per_sm; double us; };
+
+template <int NT>
+int plan_split(decxb_ctx* ctx, int64_t M, int64_t N, int num_kb, Cut* out)
+{
+    const Resident& r = resident<NT>(ctx);
+    if (r.err != cudaSuccess) return decxb_fail(ctx, DECXB_ERR_CUDA, std::string("fp8 kernel attributes: ") + cudaGetErrorString(r.err));
+    const int64_t tiles = decxb_ceil_div(M, NT) * decxb_ceil_div(N, BM_CTA);
+    int i = 3;
+    while (i > 0 && (tiles > r.clusters[i] || num_kb < (4 << i))) --i;
+    Cut c = {1 << i, 1, 0.0};
+    const int fit = r.clusters[i] > 0 ? r.clusters[i] : 1;
+    c.us = 5.0 + 0.36 * (double)decxb_ceil_div(tiles, fit) * (double)decxb_ceil_div(num_kb, c.splits);
+    if (SplitCfg<NT>::CTAS_PER_SM == 2) {
+        if (tiles > fit) c.per_sm = 2;
+        else if (i < 2 && tiles * c.splits * 5 < (int64_t)ctx->sm_count * 4 && num_kb >= (8 << i)) { c.splits *= 2; c.per_sm = 2; }
+    }
+    *out = c;
+    return DECXB_OK;
+}
+
+template <int NT>
+int launch_split(decxb_ctx* ctx, const decxb_fp8_matrix& A, const decxb_fp8_matrix& B, Params p, const Cut& cut, cudaStream_t s)
+{
+    using C = SplitCfg<NT>;
+    CUtensorMap mw, mx;
+    int rc;
+    if ((rc = make_map_fp8(ctx, &mw, B, BM_CTA)) || (rc = make_map_fp8(ctx, &mx, A, NT))) return rc;
+    const int64_t tm = decxb_ceil_div(p.M, NT), tn = decxb_ceil_div(p.N, BM_CTA);
+    if (tm * tn * cut.splits > 0x7fffffffLL) return decxb_fail(ctx, DECXB_ERR_TOO_LARGE, "fp8 gemm tiles");
+    p.tiles_m = (int)tm; p.tiles_n = (int)tn;
+    p.idesc = make_idesc_fp8(BM_CTA, NT, B.type, A.type);
+    cudaLaunchAttribute attr[2];
+    cudaLaunchConfig_t cfg = split_config<NT>(attr, tm * tn, cut.splits, cut.per_sm);
+    cfg.stream = s;
+    decxb_launch_scope scope(ctx, s, DECXB_K_GEMM);
+    DECXB_CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, decxb_gemm_fp8_split_kernel<NT>, mw, mx, p, cut.splits, C::stages(cut.per_sm)));
+    return DECXB_OK;
+}
+
+template <int NT>
+int plan_and_launch_split(decxb_ctx* ctx, const decxb_fp8_matrix& A, const decxb_fp8_matrix& B, const Params& p, cudaStream_t s)
+{
+    Cut cut;
+    const int rc = plan_split<NT>(ctx, p.M, p.N, p.num_kb, &cut);
+    return rc ? rc : launch_split<NT>(ctx, A, B, p, cut, s);
+}
+
+/* The kernel of a product: tiles of NT tokens for up to 64 tokens, otherwise what takes less, split tiles of 128 tokens or
+ * pairs' tiles of 256 x 256 (512 x 4096 x 4096: 19.1 and 18.7 us; 256 x 4096 x 4096: 13.6 and 18.3). */
+int launch_product(decxb_ctx* ctx, const decxb_fp8_matrix& A, const decxb_fp8_matrix& B, const Params& p, cudaStream_t s)
+{
+    if (p.M <= 16) return plan_and_launch_split<16>(ctx, A, B, p, s);
+    if (p.M <= 32) return plan_and_launch_split<32>(ctx, A, B, p, s);
+    if (p.M <= 64) return plan_and_launch_split<64>(ctx, A, B, p, s);
+    Cut cut;
+    if (int rc = plan_split<128>(ctx, p.M, p.N, p.num_kb, &cut)) return rc;
+    const bool by_row = B.block_rows == 1;
+    const int64_t pairs = decxb_ceil_div(p.M, 256) * decxb_ceil_div(p.N, 256), at_once = ctx->sm_count / 2 > 0 ? ctx->sm_count / 2 : 1;
+    const double pair_us = 5.0 + (by_row ? 0.75 : 0.42) * (double)decxb_ceil_div(pairs, at_once) * (double)p.num_kb;
+    if (cut.us < pair_us) return launch_split<128>(ctx, A, B, p, cut, s);
+    return by_row ? launch<true>(ctx, A, B, p, s) : launch<false>(ctx, A, B, p, s);
 }
 
 /* Codes that the copy engine cannot address are copied to a pitch it can. */
@@ -600,13 +999,9 @@ int gemm_fp8(decxb_ctx* ctx, const decxb_fp8_matrix* pa, const decxb_fp8_matrix*
         p.C = C; p.ldc = ldc; p.D = D; p.ldd = ldd; p.d_type = d_type;
         /* the copy engine clips a store at the array's edge in whole 16-byte pieces, so N has to be made of them too */
         p.tma_store = !C && aligned(D, ldd * e, 16) && N * e % 16 == 0;
+        p.d_vec = aligned(D, ldd * e, 4 * e);
         p.wait_limit_ns = ctx->wait_limit_ns; p.status = ctx->d_status;
-        const bool by_row = B.block_rows == 1;
-        const int64_t pairs = decxb_ceil_div(M, 256) * decxb_ceil_div(N, 256);
-        if (pairs * 2 >= ctx->sm_count / 2)
-            rc = by_row ? launch<2, 128, true>(ctx, A, B, p, s) : launch<2, 128, false>(ctx, A, B, p, s);
-        else
-            rc = by_row ? launch<1, 128, true>(ctx, A, B, p, s) : launch<1, 128, false>(ctx, A, B, p, s);
+        rc = launch_product(ctx, A, B, p, s);
     }
     if (a_copy) decxb_free_on_stream(ctx, a_copy, s);
     if (b_copy) decxb_free_on_stream(ctx, b_copy, s);
