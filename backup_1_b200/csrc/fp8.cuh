@@ -40,6 +40,28 @@ __device__ __forceinline__ void load8(const T* p, int n, bool vec, float* v)
     }
 }
 
+/* Eight elements as they lie in memory: what a thread keeps of a row until it needs the values. */
+template <typename T> struct Raw8 { uint4 u[sizeof(T) / 2]; };
+template <typename T>
+__device__ __forceinline__ void load_raw(const T* p, int n, bool vec, Raw8<T>& o)
+{
+    if (n >= 8 && vec) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) o.u[i] = *(reinterpret_cast<const uint4*>(p) + i);
+    } else {
+        T* e = reinterpret_cast<T*>(o.u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = j < n ? p[j] : from_f32<T>(0.0f);
+    }
+}
+template <typename T>
+__device__ __forceinline__ void unpack(const Raw8<T>& r, float* v)
+{
+    const T* e = reinterpret_cast<const T*>(r.u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = to_f32(e[j]);
+}
+
 template <typename T>
 __device__ __forceinline__ void store8(T* p, int n, bool vec, const float* v)
 {
@@ -86,14 +108,34 @@ __device__ __forceinline__ float scale_of(float amax, int type, int rule)
     return s < 1.17549435e-38f ? 1.17549435e-38f : s;
 }
 
-/* Eight codes of v * inv, rounded to nearest even; saturation only meets what the scale's own rounding pushed a
- * hair over the largest value. */
-__device__ __forceinline__ uint2 codes8(const float* v, float inv, int type)
+/* What a block's scale does to its values.  With the amax rule x / s of 16-bit x often lies half way between two codes but for
+ * the rounding of s itself, so a product with 1 / s alone, one step of fp32 off, turns four codes in ten thousand
+ * over: one correction by the remainder x - q s makes it the fp32 quotient.  With the power-of-two rule the product
+ * is exact. */
+struct Quantiser {
+    float inv, s;          /* 1 / scale, and the scale (0 for an infinite one, whose finite values give 0) */
+    bool exact;
+};
+__device__ __forceinline__ Quantiser quantiser(float scale, int rule)
+{
+    Quantiser z;
+    z.inv = __frcp_rn(scale); z.s = scale < INFINITY ? scale : 0.0f; z.exact = rule == DECXB_SCALE_POW2;
+    return z;
+}
+__device__ __forceinline__ float quotient(const Quantiser& z, float x)
+{
+    const float q = x * z.inv;
+    return z.exact ? q : fmaf(fmaf(-q, z.s, x), z.inv, q);
+}
+
+/* Eight codes, rounded to nearest even; saturation only meets what the scale's own rounding pushed a hair over the
+ * largest value. */
+__device__ __forceinline__ uint2 codes8(const float* v, const Quantiser& z, int type)
 {
     uint32_t h[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const float2 f = make_float2(v[2 * j] * inv, v[2 * j + 1] * inv);
+        const float2 f = make_float2(quotient(z, v[2 * j]), quotient(z, v[2 * j + 1]));
         h[j] = type == DECXB_FP8_E4M3 ? __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3)
                                       : __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E5M2);
     }

@@ -42,7 +42,7 @@ __device__ __forceinline__ void quantise_row8(const NormArgs& a, int64_t row, in
     for (int o = 8; o; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     if (n <= 0) return;
     const float s = scale_of(amax, a.qtype, a.rule);
-    store_codes8(a.q + row * a.ldq + c, n, a.qvec, codes8(y, __frcp_rn(s), a.qtype));
+    store_codes8(a.q + row * a.ldq + c, n, a.qvec, codes8(y, quantiser(s, a.rule), a.qtype));
     if ((c & 127) == 0) a.s[row * a.srs + (c >> 7) * a.sbs] = s;
 }
 
@@ -353,12 +353,34 @@ struct QuantArgs {
     struct Out { uint8_t* data; float* s; int64_t ld, srs, sbs; int type, block_rows; bool vec; } q, t;
 };
 
+/* Largest magnitudes of two 16-bit lanes (NaN wins) or of one float. */
+__device__ __forceinline__ uint32_t max_word(uint32_t a, uint32_t b, const __nv_bfloat16*)
+{
+    const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t max_word(uint32_t a, uint32_t b, const __half*)
+{
+    const __half2 m = __hmax2_nan(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t max_word(uint32_t a, uint32_t b, const float*) { return __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b))); }
 template <typename T>
-__global__ void __launch_bounds__(256)
+__device__ __forceinline__ uint32_t shuffle_max(uint32_t a, int o)
+{
+    return max_word(a, __shfl_xor_sync(0xffffffffu, a, o), static_cast<const T*>(nullptr));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
 decxb_quantize_fp8_kernel(const QuantArgs a)
 {
-    __shared__ float colmax[8][128];
-    __shared__ float wmax[8];
+    /* W words hold the eight columns of a row, E columns to a word; magnitudes are compared as words, two columns of 16 bits at once */
+    constexpr int W = 2 * (int)sizeof(T), E = 8 / W;
+    constexpr uint32_t MAG = E == 2 ? 0x7fff7fffu : 0x7fffffffu;
+    const T* const kind = nullptr;
+    __shared__ uint32_t colmax[8][16 * W];
+    __shared__ uint32_t wmax[8];
     __shared__ __align__(16) uint8_t tr[128 * 128];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = tid >> 4, t = tid & 15;
     const int64_t tile_r = blockIdx.x / a.tiles_c, tile_c = blockIdx.x % a.tiles_c;
@@ -366,36 +388,40 @@ decxb_quantize_fp8_kernel(const QuantArgs a)
     const int64_t row = r0 + g * 8, col = c0 + t * 8;
     const int nr = (int)max((int64_t)0, min((int64_t)8, a.rows - row));          /* rows and columns that exist here */
     const int nc = (int)max((int64_t)0, min((int64_t)8, a.cols - col));
-    float v[8][8];
+    Raw8<T> x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        load8(static_cast<const T*>(a.x) + (row + i) * a.ldx + col, i < nr ? nc : 0, a.vec, v[i]);
+    for (int i = 0; i < 8; ++i) load_raw(static_cast<const T*>(a.x) + (row + i) * a.ldx + col, i < nr ? nc : 0, a.vec, x[i]);
+    auto word = [&](int i, int k) { return reinterpret_cast<const uint32_t*>(x[i].u)[k]; };
+    auto lane_of = [&](uint32_t w, int e) -> float {      /* column e of a word */
+        if constexpr (E == 2) { const T* p = reinterpret_cast<const T*>(&w); return to_f32(p[e]); }
+        else return __uint_as_float(w);
+    };
 
     const bool whole = (a.q.data && a.q.block_rows == 128) || (a.t.data && a.t.block_rows == 128);
     const bool by_col = a.t.data && a.t.block_rows == 1;
     if (whole || by_col) {
-        float m8[8], m = 0.0f;
+        uint32_t m = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            m8[j] = fabsf(v[0][j]);
+        for (int k = 0; k < W; ++k) {
+            uint32_t c = word(0, k) & MAG;
 #pragma unroll
-            for (int i = 1; i < 8; ++i) m8[j] = max_nan(m8[j], fabsf(v[i][j]));
-            m8[j] = max_nan(m8[j], __shfl_xor_sync(0xffffffffu, m8[j], 16));
-            m = max_nan(m, m8[j]);
-        }
-        if (by_col && lane < 16) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) colmax[warp][t * 8 + j] = m8[j];
+            for (int i = 1; i < 8; ++i) c = max_word(c, word(i, k) & MAG, kind);
+            c = shuffle_max<T>(c, 16);
+            if (by_col && lane < 16) colmax[warp][t * W + k] = c;
+            m = k ? max_word(m, c, kind) : c;
         }
 #pragma unroll
-        for (int o = 8; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+        for (int o = 8; o; o >>= 1) m = shuffle_max<T>(m, o);
         if (lane == 0) wmax[warp] = m;
         __syncthreads();
     }
     float tile_max = 0.0f;
     if (whole) {
+        uint32_t m = wmax[0];
 #pragma unroll
-        for (int w = 0; w < 8; ++w) tile_max = max_nan(tile_max, wmax[w]);
+        for (int w = 1; w < 8; ++w) m = max_word(m, wmax[w], kind);
+#pragma unroll
+        for (int e = 0; e < E; ++e) tile_max = max_nan(tile_max, lane_of(m, e));
     }
 
     if (a.q.data) {
@@ -405,15 +431,19 @@ decxb_quantize_fp8_kernel(const QuantArgs a)
         for (int i = 0; i < 8; ++i) {
             float s = st;
             if (a.q.block_rows == 1) {
-                float m = 0.0f;
+                uint32_t m = word(i, 0) & MAG;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) m = max_nan(m, fabsf(v[i][j]));
+                for (int k = 1; k < W; ++k) m = max_word(m, word(i, k) & MAG, kind);
+                float f = lane_of(m, 0);
+                if (E == 2) f = max_nan(f, lane_of(m, E - 1));
 #pragma unroll
-                for (int o = 8; o; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-                s = scale_of(m, a.q.type, a.rule);
+                for (int o = 8; o; o >>= 1) f = max_nan(f, __shfl_xor_sync(0xffffffffu, f, o));
+                s = scale_of(f, a.q.type, a.rule);
                 if (t == 0 && i < nr) a.q.s[(row + i) * a.q.srs + tile_c * a.q.sbs] = s;
             }
-            if (i < nr && nc > 0) store_codes8(a.q.data + (row + i) * a.q.ld + col, nc, a.q.vec, codes8(v[i], __frcp_rn(s), a.q.type));
+            float v[8];
+            unpack(x[i], v);
+            if (i < nr && nc > 0) store_codes8(a.q.data + (row + i) * a.q.ld + col, nc, a.q.vec, codes8(v, quantiser(s, a.rule), a.q.type));
         }
     }
 
@@ -421,19 +451,26 @@ decxb_quantize_fp8_kernel(const QuantArgs a)
         const float st = a.t.block_rows == 128 ? scale_of(tile_max, a.t.type, a.rule) : 0.0f;
         if (a.t.block_rows == 128 && tid == 0) a.t.s[tile_c * a.t.srs + tile_r * a.t.sbs] = st;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            float s = st;
+        for (int k = 0; k < W; ++k) {
+            uint32_t m = 0;
             if (by_col) {
-                float m = 0.0f;
+                m = colmax[0][t * W + k];
 #pragma unroll
-                for (int w = 0; w < 8; ++w) m = max_nan(m, colmax[w][t * 8 + j]);
-                s = scale_of(m, a.t.type, a.rule);
-                if (g == 0 && j < nc) a.t.s[(col + j) * a.t.srs + tile_r * a.t.sbs] = s;
+                for (int w = 1; w < 8; ++w) m = max_word(m, colmax[w][t * W + k], kind);
             }
-            float w8[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) w8[i] = v[i][j];
-            *reinterpret_cast<uint2*>(tr + (t * 8 + j) * 128 + ((g ^ t) << 3)) = codes8(w8, __frcp_rn(s), a.t.type);
+            for (int e = 0; e < E; ++e) {
+                const int j = k * E + e;
+                float s = st;
+                if (by_col) {
+                    s = scale_of(lane_of(m, e), a.t.type, a.rule);
+                    if (g == 0 && j < nc) a.t.s[(col + j) * a.t.srs + tile_r * a.t.sbs] = s;
+                }
+                float v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = lane_of(word(i, k), e);
+                *reinterpret_cast<uint2*>(tr + (t * 8 + j) * 128 + ((g ^ t) << 3)) = codes8(v, quantiser(s, a.rule), a.t.type);
+            }
         }
         __syncthreads();
         /* out: row c of the transpose, eight of X's rows per thread, 16 lanes a row */

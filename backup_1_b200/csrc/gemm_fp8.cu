@@ -157,14 +157,28 @@ __device__ __forceinline__ float4 lds_f32x4(uint32_t at)
     float4 v; asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory"); return v;
 }
 
-/* tcgen05.wait::ld with the loaded registers as operands: nothing that reads them can be moved ahead of it. */
-__device__ __forceinline__ void tmem_ld_wait32(float* v)
+/* 16 lanes x 8 G columns: register 4 g + k is column 8 g + 2 (lane % 4) + (k & 1) of lane lane / 4 + 8 (k >> 1). */
+template <int G>
+__device__ __forceinline__ void tmem_ld_16x256(uint32_t taddr, float* v)
 {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]),
-                   "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]) :: "memory");
-    asm volatile("" : "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]),
-                      "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31]) :: "memory");
+    if constexpr (G == 1)
+        asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(taddr) : "memory");
+    else if constexpr (G == 2)
+        asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "r"(taddr) : "memory");
+    else
+        asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
+                       "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]) : "r"(taddr) : "memory");
+}
+/* tcgen05.wait::ld with the loaded registers as operands: nothing that reads them can be moved ahead of it. */
+template <int N>
+__device__ __forceinline__ void tmem_ld_wait_n(float* v)
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]) :: "memory");
+#pragma unroll
+    for (int i = 4; i < N; ++i) asm volatile("" : "+f"(v[i]) :: "memory");
 }
 
 /* Tile order: groups of `group` tile-rows, column by column inside a group (operand panels shared in L2). */
@@ -194,6 +208,31 @@ __device__ __forceinline__ void box_pieces(uint32_t box, int lane, int first, co
         const uint32_t at = box + (uint32_t)lane * 128u + (uint32_t)(((first + j / E) ^ (lane & 7)) << 4);
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(at), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
     }
+}
+
+/* The same from registers in the 16x256b shape (two lane halves of four groups of eight columns). */
+template <typename T>
+__device__ __forceinline__ void box_fragments(uint32_t box, int lane, int first, const float* v)
+{
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+        const int r = (i >> 4) * 16 + ((i >> 1) & 1) * 8 + (lane >> 2), g = (i >> 2) & 3;
+        const uint32_t row = box + (uint32_t)r * 128u;
+        if constexpr (sizeof(T) == 4) {
+            const uint32_t at = row + (uint32_t)(((2 * g + ((lane & 3) >> 1)) ^ (r & 7)) << 4) + (uint32_t)(lane & 1) * 8u;
+            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" :: "r"(at), "f"(v[i]), "f"(v[i + 1]) : "memory");
+        } else {
+            alignas(4) T e[2] = {from_f32<T>(v[i]), from_f32<T>(v[i + 1])};
+            const uint32_t at = row + (uint32_t)(((first + g) ^ (r & 7)) << 4) + (uint32_t)(lane & 3) * 4u;
+            asm volatile("st.shared.b32 [%0], %1;" :: "r"(at), "r"(*reinterpret_cast<const uint32_t*>(e)) : "memory");
+        }
+    }
+}
+template <typename T, bool FRAGMENTS>
+__device__ __forceinline__ void box_write(uint32_t box, int lane, int first, const float* v)
+{
+    if constexpr (FRAGMENTS) box_fragments<T>(box, lane, first, v);
+    else                     box_pieces<T>(box, lane, first, v);
 }
 
 /* By the threads, row after row with one column a lane: any address and pitch, and the addend on the way. */
@@ -425,29 +464,44 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                 const int acc = unit % C::BUFS;
                 if (!warp_wait(sfull_bar(slot), sphase, p, 1600 + slot, t)) { alive = false; break; }
                 const uint32_t sc = ring + (uint32_t)(slot * C::KB_FLOATS) * 4u;
-                float sr = lds_f32(sc + (uint32_t)(q * 32 + lane) * 4u);
-                if (!COLVEC) sr *= lds_f32(sc + (uint32_t)(BM_CTA + eh) * 4u);
+                /* this thread's rows: one, or with a factor per column the four of the 16x256b shape */
+                float sr[COLVEC ? 4 : 1];
+                if constexpr (COLVEC) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sr[i] = lds_f32(sc + (uint32_t)(q * 32 + i * 8 + (lane >> 2)) * 4u);
+                } else {
+                    sr[0] = lds_f32(sc + (uint32_t)(q * 32 + lane) * 4u) * lds_f32(sc + (uint32_t)(BM_CTA + eh) * 4u);
+                }
                 if (!warp_wait(done_bar(stage), phase, p, 1400 + stage, t)) { alive = false; break; }
                 tc_fence_after();
                 /* 32 columns are multiplied while the next 32 are on their way */
                 float v[2][32];
-                tmem_ld_32x32(tlane + (uint32_t)(acc * C::UMMA_N), v[0]);
+                const uint32_t tacc = tlane + (uint32_t)(acc * C::UMMA_N);
+                auto load32 = [&](int c, float* w) {
+                    if constexpr (COLVEC) {
+                        tmem_ld_16x256<4>(tacc + (uint32_t)c, w);
+                        tmem_ld_16x256<4>(tacc + (16u << 16) + (uint32_t)c, w + 16);
+                    } else tmem_ld_32x32(tacc + (uint32_t)c, w);
+                };
+                load32(0, v[0]);
 #pragma unroll
                 for (int c = 0; c < C::ACC; c += 32) {
                     float* w = v[(c >> 5) & 1];
-                    tmem_ld_wait32(w);
-                    if (c + 32 < C::ACC) tmem_ld_32x32(tlane + (uint32_t)(acc * C::UMMA_N + c + 32), v[((c >> 5) + 1) & 1]);
+                    tmem_ld_wait_n<32>(w);
+                    if (c + 32 < C::ACC) load32(c + 32, v[((c >> 5) + 1) & 1]);
+                    if constexpr (COLVEC) {
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        float4 f = make_float4(sr, sr, sr, sr);
-                        if (COLVEC) {
-                            const float4 g = lds_f32x4(sc + (uint32_t)(BM_CTA + eh * C::ACC + c + j) * 4u);
-                            f.x *= g.x; f.y *= g.y; f.z *= g.z; f.w *= g.w;
+                        for (int g = 0; g < 4; ++g) {
+                            const float2 x = lds_f32x2(sc + (uint32_t)(BM_CTA + eh * C::ACC + c + g * 8 + (lane & 3) * 2) * 4u);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const int j = (i >> 2) * 16 + g * 4 + (i & 3);
+                                sum[c + j] = fmaf(w[j], sr[i >> 1] * ((i & 1) ? x.y : x.x), sum[c + j]);
+                            }
                         }
-                        sum[c + j] = fmaf(w[j], f.x, sum[c + j]);
-                        sum[c + j + 1] = fmaf(w[j + 1], f.y, sum[c + j + 1]);
-                        sum[c + j + 2] = fmaf(w[j + 2], f.z, sum[c + j + 2]);
-                        sum[c + j + 3] = fmaf(w[j + 3], f.w, sum[c + j + 3]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) sum[c + j] = fmaf(w[j], sr[0], sum[c + j]);
                     }
                 }
                 /* block taken: hand the buffer (in the leader CTA) and the scales' slot back */
@@ -477,9 +531,9 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                         if (lane == 0) tma_store_wait_read<0>();      /* the box before has been read */
                         __syncwarp();
                     }
-                    if (!narrow)                        box_pieces<float>(box, lane, 0, v);
-                    else if (p.d_type == DECXB_F16)     box_pieces<__half>(box, lane, first, v);
-                    else                                box_pieces<__nv_bfloat16>(box, lane, first, v);
+                    if (!narrow)                        box_write<float, COLVEC>(box, lane, 0, v);
+                    else if (p.d_type == DECXB_F16)     box_write<__half, COLVEC>(box, lane, first, v);
+                    else                                box_write<__nv_bfloat16, COLVEC>(box, lane, first, v);
                     if (!narrow || first || col0 + c + 32 >= p.N) {
                         fence_proxy_async_smem();
                         __syncwarp();
@@ -490,7 +544,7 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                     }
                 } else {
                     __syncwarp();
-                    box_pieces<float>(box, lane, 0, v);
+                    box_write<float, COLVEC>(box, lane, 0, v);
                     __syncwarp();
                     if (!narrow)                        box_rows<float>(p, box, lane, row0, col0 + c + lane);
                     else if (p.d_type == DECXB_F16)     box_rows<__half>(p, box, lane, row0, col0 + c + lane);
@@ -543,30 +597,6 @@ struct SplitCfg {
     static_assert(BUFS >= 2, "buffers");
     static_assert(NT * PITCH * 4 <= stages(CTAS_PER_SM) * STAGE_BYTES, "partial sums reuse the stages");
 };
-
-/* 16 lanes x 8 G columns: register 4 g + k is column 8 g + 2 (lane % 4) + (k & 1) of lane lane / 4 + 8 (k >> 1). */
-template <int G>
-__device__ __forceinline__ void tmem_ld_16x256(uint32_t taddr, float* v)
-{
-    if constexpr (G == 1)
-        asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0, %1, %2, %3}, [%4];"
-                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(taddr) : "memory");
-    else if constexpr (G == 2)
-        asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "r"(taddr) : "memory");
-    else
-        asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
-                       "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]) : "r"(taddr) : "memory");
-}
-/* tcgen05.wait::ld with n loaded registers as operands (see tmem_ld_wait32). */
-template <int N>
-__device__ __forceinline__ void tmem_ld_wait_n(float* v)
-{
-    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]) :: "memory");
-#pragma unroll
-    for (int i = 4; i < N; ++i) asm volatile("" : "+f"(v[i]) :: "memory");
-}
 
 template <int NT>
 __global__ void __launch_bounds__(THREADS, SplitCfg<NT>::CTAS_PER_SM)
@@ -902,7 +932,8 @@ int plan_split(decxb_ctx* ctx, int64_t M, int64_t N, int num_kb, Cut* out)
     while (i > 0 && (tiles > r.clusters[i] || num_kb < (4 << i))) --i;
     Cut c = {1 << i, 1, 0.0};
     const int fit = r.clusters[i] > 0 ? r.clusters[i] : 1;
-    c.us = 5.0 + 0.36 * (double)decxb_ceil_div(tiles, fit) * (double)decxb_ceil_div(num_kb, c.splits);
+    const int64_t waves = decxb_ceil_div(tiles, fit);
+    c.us = 5.0 + (waves > 1 ? 0.50 : 0.36) * (double)waves * (double)decxb_ceil_div(num_kb, c.splits);
     if (SplitCfg<NT>::CTAS_PER_SM == 2) {
         if (tiles > fit) c.per_sm = 2;
         else if (i < 2 && tiles * c.splits * 5 < (int64_t)ctx->sm_count * 4 && num_kb >= (8 << i)) { c.splits *= 2; c.per_sm = 2; }
@@ -949,7 +980,7 @@ int launch_product(decxb_ctx* ctx, const decxb_fp8_matrix& A, const decxb_fp8_ma
     if (int rc = plan_split<128>(ctx, p.M, p.N, p.num_kb, &cut)) return rc;
     const bool by_row = B.block_rows == 1;
     const int64_t pairs = decxb_ceil_div(p.M, 256) * decxb_ceil_div(p.N, 256), at_once = ctx->sm_count / 2 > 0 ? ctx->sm_count / 2 : 1;
-    const double pair_us = 5.0 + (by_row ? 0.75 : 0.42) * (double)decxb_ceil_div(pairs, at_once) * (double)p.num_kb;
+    const double pair_us = 5.0 + (by_row ? 0.80 : 0.42) * (double)decxb_ceil_div(pairs, at_once) * (double)p.num_kb;
     if (cut.us < pair_us) return launch_split<128>(ctx, A, B, p, cut, s);
     return by_row ? launch<true>(ctx, A, B, p, s) : launch<false>(ctx, A, B, p, s);
 }

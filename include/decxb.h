@@ -326,8 +326,8 @@ DECXB_API int decxb_gemm_fp8(decxb_ctx* ctx, const decxb_fp8_matrix* A, const de
 
 /* Quantises X [rows][cols] of x_type: Q (rows x cols) and Qt (cols x rows, the transpose, its blocks
  * running along X's rows) where given, at least one of the two.  Per block: scale by `scale_rule`,
- * at least 2^-126 (a block of zeros has that scale and zero codes); code = x * (1 / scale) rounded to
- * nearest even.  A block that holds a NaN has scale and codes NaN; one that holds an infinity has
+ * at least 2^-126 (a block of zeros has that scale and zero codes); code = the fp32 quotient x / scale,
+ * rounded to nearest even.  A block that holds a NaN has scale and codes NaN; one that holds an infinity has
  * scale infinity, its finite values give 0 and its infinities NaN.  cols may be 0 or rows may be 0:
  * nothing is written.  Bytes of Q between cols and ld are left as they were. */
 DECXB_API int decxb_quantize_fp8(decxb_ctx* ctx, int x_type, int64_t rows, int64_t cols, const void* X, int64_t ldx,
