@@ -97,9 +97,13 @@ __device__ __forceinline__ float max_nan(float a, float b)
     float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r;
 }
 
+/* amax / largest value, correctly rounded (a product with the reciprocal and one correction by the remainder), then the
+ * rule; infinity and NaN pass. */
 __device__ __forceinline__ float scale_of(float amax, int type, int rule)
 {
-    float s = __fdiv_rn(amax, type == DECXB_FP8_E4M3 ? 448.0f : 57344.0f);
+    const float most = type == DECXB_FP8_E4M3 ? 448.0f : 57344.0f, inv = type == DECXB_FP8_E4M3 ? 1.0f / 448.0f : 1.0f / 57344.0f;
+    const float q = amax * inv;
+    float s = amax < INFINITY ? fmaf(fmaf(-q, most, amax), inv, q) : amax;
     if (rule == DECXB_SCALE_POW2) {
         /* up to the next power of two: exponent + 1 unless the mantissa is zero (infinity and NaN stay) */
         const uint32_t u = __float_as_uint(s);
@@ -110,34 +114,29 @@ __device__ __forceinline__ float scale_of(float amax, int type, int rule)
 
 /* What a block's scale does to its values.  With the amax rule x / s of 16-bit x often lies half way between two codes but for
  * the rounding of s itself, so a product with 1 / s alone, one step of fp32 off, turns four codes in ten thousand
- * over: one correction by the remainder x - q s makes it the fp32 quotient.  With the power-of-two rule the product
- * is exact. */
-struct Quantiser {
-    float inv, s;          /* 1 / scale, and the scale (0 for an infinite one, whose finite values give 0) */
-    bool exact;
-};
-__device__ __forceinline__ Quantiser quantiser(float scale, int rule)
+ * over: one correction by the remainder x - q s makes it the fp32 quotient.  (With the power-of-two rule the product is
+ * exact and the remainder 0.) */
+struct Quantiser { float inv, s; };          /* 1 / scale, and the scale (0 for an infinite one, whose finite values give 0) */
+__device__ __forceinline__ Quantiser quantiser(float scale)
 {
-    Quantiser z;
-    z.inv = __frcp_rn(scale); z.s = scale < INFINITY ? scale : 0.0f; z.exact = rule == DECXB_SCALE_POW2;
-    return z;
-}
-__device__ __forceinline__ float quotient(const Quantiser& z, float x)
-{
-    const float q = x * z.inv;
-    return z.exact ? q : fmaf(fmaf(-q, z.s, x), z.inv, q);
+    return Quantiser{__frcp_rn(scale), scale < INFINITY ? scale : 0.0f};
 }
 
 /* Eight codes, rounded to nearest even; saturation only meets what the scale's own rounding pushed a hair over the
  * largest value. */
-__device__ __forceinline__ uint2 codes8(const float* v, const Quantiser& z, int type)
+template <int TYPE>
+__device__ __forceinline__ uint2 codes8(const float* v, const Quantiser& z)
 {
     uint32_t h[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const float2 f = make_float2(quotient(z, v[2 * j]), quotient(z, v[2 * j + 1]));
-        h[j] = type == DECXB_FP8_E4M3 ? __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3)
-                                      : __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E5M2);
+        float q[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            q[e] = v[2 * j + e] * z.inv;
+            q[e] = fmaf(fmaf(-q[e], z.s, v[2 * j + e]), z.inv, q[e]);
+        }
+        h[j] = __nv_cvt_float2_to_fp8x2(make_float2(q[0], q[1]), __NV_SATFINITE, TYPE == DECXB_FP8_E4M3 ? __NV_E4M3 : __NV_E5M2);
     }
     return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
 }
@@ -146,8 +145,8 @@ __device__ __forceinline__ void store_codes8(uint8_t* p, int n, bool vec, uint2 
 {
     if (n >= 8 && vec) *reinterpret_cast<uint2*>(p) = c;
     else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) if (j < n) p[j] = (uint8_t)((j < 4 ? c.x : c.y) >> (8 * (j & 3)));
+#pragma unroll 1
+        for (int j = 0; j < n && j < 8; ++j) p[j] = (uint8_t)((j < 4 ? c.x : c.y) >> (8 * (j & 3)));
     }
 }
 

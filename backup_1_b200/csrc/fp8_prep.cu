@@ -4,7 +4,9 @@
  * All of them are bound by memory: every array is read once and written once.
  */
 #include "fp8.cuh"
+#include "tc_ptx.cuh"
 
+#include <mutex>
 #include <new>
 
 namespace {
@@ -18,9 +20,31 @@ __device__ __forceinline__ float warp_sum(float v)
     return v;
 }
 
+/* Every kernel here may start while the one before it in the stream drains, and waits for its memory here. */
+__device__ __forceinline__ void start_after_previous()
+{
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+template <typename... P, typename... A>
+int launch_after(decxb_ctx* ctx, void (*kernel)(P...), unsigned grid, dim3 threads, size_t smem, cudaStream_t s, const A&... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid, 1, 1); cfg.blockDim = threads; cfg.dynamicSmemBytes = smem; cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr; cfg.numAttrs = 1;
+    decxb_launch_scope scope(ctx, s, DECXB_K_SPLIT);
+    DECXB_CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, kernel, args...));
+    return DECXB_OK;
+}
+
 /* ---- root-mean-square norm ---------------------------------------------------------------
- * One block per row.  A thread holds VPT vectors of eight consecutive columns, vector i * blockDim + tid, so the
- * 16 lanes of half a warp cover one 128-column block of the row and its largest magnitude is four shuffles away. */
+ * One block per row, or eight rows of up to 256 columns with a warp each.  A thread holds VPT vectors of eight consecutive
+ * columns, vector i * blockDim + tid, so the 16 lanes of half a warp cover one 128-column block of the row and its
+ * largest magnitude is four shuffles away. */
 struct NormArgs {
     int64_t rows, cols;
     const void *x, *r, *gamma; void *h, *y;
@@ -31,64 +55,82 @@ struct NormArgs {
     uint8_t* q; int64_t ldq; float* s; int64_t srs, sbs; int qtype; bool qvec;
 };
 
-/* Quantises eight columns from `c` on of one row: the 16 lanes of the block agree on its scale. */
-__device__ __forceinline__ void quantise_row8(const NormArgs& a, int64_t row, int64_t c, const float* y)
+/* Quantises the `n` columns (eight, but at a ragged row's end) from `c` on of one row: the 16 lanes of the block agree on its scale. */
+__device__ __forceinline__ void quantise_row8(const NormArgs& a, uint8_t* q, float* scales, int c, int n, const float* y)
 {
-    const int n = (int)min((int64_t)8, a.cols - c);
-    float amax = 0.0f;
+    float amax = fabsf(y[0]);                  /* columns that do not exist are zeros */
 #pragma unroll
-    for (int j = 0; j < 8; ++j) amax = max_nan(amax, j < n ? fabsf(y[j]) : 0.0f);
+    for (int j = 1; j < 8; ++j) amax = max_nan(amax, fabsf(y[j]));
 #pragma unroll
     for (int o = 8; o; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     if (n <= 0) return;
     const float s = scale_of(amax, a.qtype, a.rule);
-    store_codes8(a.q + row * a.ldq + c, n, a.qvec, codes8(y, quantiser(s, a.rule), a.qtype));
-    if ((c & 127) == 0) a.s[row * a.srs + (c >> 7) * a.sbs] = s;
+    const Quantiser z = quantiser(s);
+    store_codes8(q + c, n, a.qvec, a.qtype == DECXB_FP8_E4M3 ? codes8<DECXB_FP8_E4M3>(y, z) : codes8<DECXB_FP8_E5M2>(y, z));
+    if ((c & 127) == 0) scales[(c >> 7) * a.sbs] = s;
 }
 
-template <typename T, int VPT>
-__global__ void __launch_bounds__(1024)
+/* WHOLE: every vector of the row lies in it and every array takes 128-bit accesses (the checks cost a third of the kernel's
+ * instructions, which bound it for 16-bit types). */
+template <typename T, int VPT, bool WHOLE>
+__global__ void __launch_bounds__(1024, VPT <= 2 ? 2 : 1)
 decxb_rmsnorm_kernel(const NormArgs a)
 {
     __shared__ float part[32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nwarps = blockDim.x >> 5;
-    const int64_t row = blockIdx.x;
+    const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+    const int cols = (int)a.cols;
+    if (row >= a.rows) return;             /* a whole warp, in a block without barriers */
+    const bool vec = WHOLE || a.vec, gvec = WHOLE || a.gvec;
+    auto count = [&](int c) { return WHOLE ? (c < cols ? 8 : 0) : min(8, cols - c); };
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
-    const T* r = a.r ? static_cast<const T*>(a.r) + row * a.ldr : nullptr;
     float v[VPT][8];
     float sum = 0.0f;
+    start_after_previous();
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-        const int64_t c = ((int64_t)i * blockDim.x + tid) * 8;
-        const int n = (int)min((int64_t)8, a.cols - c);
-        load8(x + c, n, a.vec, v[i]);
-        if (r) {
+        const int c = (i * (int)blockDim.x + tid) * 8;
+        load8(x + c, count(c), vec, v[i]);
+    }
+    if (a.r) {
+        const T* r = static_cast<const T*>(a.r) + row * a.ldr;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int c = (i * (int)blockDim.x + tid) * 8;
             float w[8];
-            load8(r + c, n, a.vec, w);
+            load8(r + c, count(c), vec, w);
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[i][j] += w[j];
         }
+    }
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum = fmaf(v[i][j], v[i][j], sum);
-    }
     sum = warp_sum(sum);
     if (nwarps > 1) {
         if (lane == 0) part[warp] = sum;
         __syncthreads();
         sum = warp_sum(lane < nwarps ? part[lane] : 0.0f);
     }
-    const float rstd = rsqrtf(sum / (float)a.cols + a.eps);
+    const float rstd = rsqrtf(sum / (float)cols + a.eps);
+    if (a.h) {
+        T* h = static_cast<T*>(a.h) + row * a.ldh;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int c = (i * (int)blockDim.x + tid) * 8;
+            if (count(c) > 0) store8(h + c, count(c), vec, v[i]);
+        }
+    }
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-        const int64_t c = ((int64_t)i * blockDim.x + tid) * 8;
-        const int n = (int)min((int64_t)8, a.cols - c);
-        if (a.h && n > 0) store8(static_cast<T*>(a.h) + row * a.ldh + c, n, a.vec, v[i]);
+        const int c = (i * (int)blockDim.x + tid) * 8;
         float g[8];
-        load8_any(a.gamma, a.gamma_type, c, n, a.gvec, g);
+        load8_any(a.gamma, a.gamma_type, c, count(c), gvec, g);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] = v[i][j] * rstd * g[j];
-        if (a.y && n > 0) store8(static_cast<T*>(a.y) + row * a.ldy + c, n, a.vec, v[i]);
-        if (a.q) quantise_row8(a, row, c, v[i]);
+        if (a.y && count(c) > 0) store8(static_cast<T*>(a.y) + row * a.ldy + c, count(c), vec, v[i]);
+        if (a.q) quantise_row8(a, a.q + row * a.ldq, a.s + row * a.srs, c, count(c), v[i]);
     }
 }
 
@@ -102,6 +144,7 @@ decxb_rmsnorm_wide_kernel(const NormArgs a)
     const int64_t row = blockIdx.x;
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     const T* r = a.r ? static_cast<const T*>(a.r) + row * a.ldr : nullptr;
+    start_after_previous();
     float sum = 0.0f, v[8], w[8];
     for (int64_t c = (int64_t)tid * 8; c < a.cols; c += (int64_t)blockDim.x * 8) {
         const int n = (int)min((int64_t)8, a.cols - c);
@@ -134,7 +177,7 @@ decxb_rmsnorm_wide_kernel(const NormArgs a)
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = v[j] * rstd * w[j];
         if (a.y && n > 0) store8(static_cast<T*>(a.y) + row * a.ldy + c, n, a.vec, v);
-        if (a.q) quantise_row8(a, row, c, v);
+        if (a.q) quantise_row8(a, a.q + row * a.ldq, a.s + row * a.srs, (int)c, n, v);
     }
 }
 
@@ -145,24 +188,32 @@ int threads_for(int64_t nvec, int vpt, int most)
     return (int)(t > most ? most : t < 32 ? 32 : t);
 }
 
+template <typename T, int VPT>
+int launch_norm_rows(decxb_ctx* ctx, const NormArgs& a, int64_t nvec, cudaStream_t s)
+{
+    const bool whole = a.vec && a.gvec && a.cols % 8 == 0 && (!a.q || a.qvec);
+    const unsigned threads = (unsigned)threads_for(nvec, VPT, 1024), rows = threads == 32 ? 8 : 1;
+    const unsigned grid = (unsigned)decxb_ceil_div(a.rows, rows);
+    return whole ? launch_after(ctx, decxb_rmsnorm_kernel<T, VPT, true>, grid, dim3(threads, rows), 0, s, a)
+                 : launch_after(ctx, decxb_rmsnorm_kernel<T, VPT, false>, grid, dim3(threads, rows), 0, s, a);
+}
+
+/* One vector a thread as far as 1024 threads reach (8192 x 4096 bf16 with one, two, four: 64, 69, 74 us): a block's loads,
+ * sum and stores follow one another, so it is the number of blocks on an SM that keeps the memory busy. */
 template <typename T>
 int launch_norm(decxb_ctx* ctx, const NormArgs& a, cudaStream_t s)
 {
     const int64_t nvec = decxb_ceil_div(a.cols, 8);
-    decxb_launch_scope scope(ctx, s, DECXB_K_SPLIT);
-    const unsigned grid = (unsigned)a.rows;
-    if (nvec <= 512)       decxb_rmsnorm_kernel<T, 1><<<grid, threads_for(nvec, 1, 512), 0, s>>>(a);
-    else if (nvec <= 1024) decxb_rmsnorm_kernel<T, 2><<<grid, threads_for(nvec, 2, 512), 0, s>>>(a);
-    else if (nvec <= 4096) decxb_rmsnorm_kernel<T, 4><<<grid, threads_for(nvec, 4, 1024), 0, s>>>(a);
-    else                   decxb_rmsnorm_wide_kernel<T><<<grid, 1024, 0, s>>>(a);
-    DECXB_CUDA_TRY(ctx, cudaGetLastError());
-    return DECXB_OK;
+    if (nvec <= 1024) return launch_norm_rows<T, 1>(ctx, a, nvec, s);
+    if (nvec <= 2048) return launch_norm_rows<T, 2>(ctx, a, nvec, s);
+    if (nvec <= 4096) return launch_norm_rows<T, 4>(ctx, a, nvec, s);
+    return launch_after(ctx, decxb_rmsnorm_wide_kernel<T>, (unsigned)a.rows, 1024, 0, s, a);
 }
 
 /* ---- its backward pass ---------------------------------------------------------------------
- * A block walks rows blockIdx, blockIdx + gridDim, ...; a thread keeps the same columns throughout and sums their share
- * of dgamma in registers.  Each block leaves its sums in its own row of the workspace, and a second kernel adds
- * the rows in ascending order: no atomics, the same bits every time. */
+ * A thread keeps the same columns throughout and sums their share of dgamma in registers.  Each block leaves its sums in
+ * its own row of the workspace, and a second kernel adds the rows in ascending order: no atomics, the same bits every
+ * time.  Rows up to 256 columns belong to a warp, longer ones to a block. */
 struct NormBwdArgs {
     int64_t rows, cols;
     const void *dy, *h, *dr, *gamma; void* dx;
@@ -177,88 +228,169 @@ struct NormBwdArgs {
 __device__ __forceinline__ float2 block_sum2(float a, float b, float2* buf, int warp, int lane, int nwarps)
 {
     a = warp_sum(a); b = warp_sum(b);
-    if (nwarps == 1) return make_float2(a, b);
     if (lane == 0) buf[warp] = make_float2(a, b);
     __syncthreads();
     const float2 p = lane < nwarps ? buf[lane] : make_float2(0.0f, 0.0f);
     return make_float2(warp_sum(p.x), warp_sum(p.y));
 }
 
-template <typename T, int VPT>
-__global__ void __launch_bounds__(512)
-decxb_rmsnorm_backward_kernel(const NormBwdArgs a)
+/* dX of eight columns, and their share of dgamma on top of `acc`: w = dY, o = dR on entry and dX on return. */
+__device__ __forceinline__ void backward8(const float* w, const float* x, const float* g, float r, float k, float* o, float* acc)
 {
-    __shared__ float2 buf[2][32];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nwarps = blockDim.x >> 5;
-    float acc[VPT][8];
 #pragma unroll
-    for (int i = 0; i < VPT; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[i][j] = 0.0f;
-    int turn = 0;
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
-        const T* dy = static_cast<const T*>(a.dy) + row * a.lddy;
-        const T* h = static_cast<const T*>(a.h) + row * a.ldh;
-        float w[VPT][8], x[VPT][8];
-        float sq = 0.0f, dot = 0.0f;
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const int64_t c = ((int64_t)i * blockDim.x + tid) * 8;
-            const int n = (int)min((int64_t)8, a.cols - c);
-            load8(dy + c, n, a.vec, w[i]);
-            load8(h + c, n, a.vec, x[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const int64_t c = ((int64_t)i * blockDim.x + tid) * 8;
-            const int n = (int)min((int64_t)8, a.cols - c);
-            float g[8];
-            load8_any(a.gamma, a.gamma_type, c, n, a.gvec, g);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                sq = fmaf(x[i][j], x[i][j], sq);
-                dot = fmaf(w[i][j] * g[j], x[i][j], dot);
-            }
-        }
-        const float2 s = block_sum2(sq, dot, buf[turn], warp, lane, nwarps);
-        const float r = rsqrtf(s.x / (float)a.cols + a.eps);
-        const float k = r * r * (s.y / (float)a.cols);
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const int64_t c = ((int64_t)i * blockDim.x + tid) * 8;
-            const int n = (int)min((int64_t)8, a.cols - c);
-            if (n <= 0) continue;
-            float g[8], o[8];
-            load8_any(a.gamma, a.gamma_type, c, n, a.gvec, g);
-            if (a.dr) load8(static_cast<const T*>(a.dr) + row * a.lddr + c, n, a.vec, o);
-            else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) o[j] = 0.0f;
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                acc[i][j] = fmaf(w[i][j], x[i][j] * r, acc[i][j]);
-                o[j] = fmaf(r, w[i][j] * g[j] - x[i][j] * k, o[j]);
-            }
-            store8(static_cast<T*>(a.dx) + row * a.lddx + c, n, a.vec, o);
-        }
-    }
-    if (!a.part) return;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-        const int64_t c = ((int64_t)i * blockDim.x + tid) * 8;
-        const int n = (int)min((int64_t)8, a.cols - c);
-        if (n > 0) store8(a.part + (int64_t)blockIdx.x * a.cols + c, n, a.cols % 4 == 0, acc[i]);
+    for (int j = 0; j < 8; ++j) {
+        acc[j] = fmaf(w[j], x[j] * r, acc[j]);
+        o[j] = fmaf(r, w[j] * g[j] - x[j] * k, o[j]);
     }
 }
 
-/* Rows too long for the registers: each row is read twice and the sums for dgamma live in the workspace. */
+/* Bulk copy of `bytes` (a multiple of 16, both addresses too) to shared memory, counted on an mbarrier. */
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 :: "r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+/* Wait for a stage's copies; where they do not come within the limit, the status word says so and the wait ends. */
+__device__ __forceinline__ void wait_copy(uint32_t bar, uint32_t parity, long long limit_ns, decxb_dev_status* status)
+{
+    unsigned long long t0 = 0;
+    for (uint32_t spins = 1; !tcptx::mbar_try_wait(bar, parity); ++spins) {
+        if (spins & 1023u) continue;
+        const unsigned long long t = tcptx::globaltimer_ns();
+        if (t0 == 0) t0 = t;
+        if ((long long)(t - t0) > limit_ns) {
+            if (atomicCAS(&status->code, 0, DECXB_DEVERR_WAIT_EXPIRED) == 0) {
+                status->where = 3000; status->block = (int)blockIdx.x; status->detail = 0;
+                __threadfence_system();
+            }
+            return;
+        }
+    }
+}
+
+/* A warp per row, eight rows a block at a time. */
+template <typename T>
+__global__ void __launch_bounds__(256, 4)
+decxb_rmsnorm_backward_kernel(const NormBwdArgs a)
+{
+    __shared__ float sums[8][256];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cols = (int)a.cols, first = lane * 8, count = min(8, cols - first);
+    float acc[8] = {}, g[8];
+    start_after_previous();
+    load8_any(a.gamma, a.gamma_type, first, count, a.gvec, g);
+    for (int64_t row = (int64_t)blockIdx.x * 8 + warp; row < a.rows; row += (int64_t)gridDim.x * 8) {
+        float w[8], x[8], o[8];
+        load8(static_cast<const T*>(a.dy) + row * a.lddy + first, count, a.vec, w);
+        load8(static_cast<const T*>(a.h) + row * a.ldh + first, count, a.vec, x);
+        load8(static_cast<const T*>(a.dr) + row * a.lddr + first, a.dr ? count : 0, a.vec, o);
+        float sq = 0.0f, dot = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { sq = fmaf(x[j], x[j], sq); dot = fmaf(w[j] * g[j], x[j], dot); }
+        const float r = rsqrtf(warp_sum(sq) / (float)cols + a.eps), k = r * r * (warp_sum(dot) / (float)cols);
+        backward8(w, x, g, r, k, o, acc);
+        if (count > 0) store8(static_cast<T*>(a.dx) + row * a.lddx + first, count, a.vec, o);
+    }
+    if (!a.part) return;
+    *reinterpret_cast<float4*>(&sums[warp][first]) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    *reinterpret_cast<float4*>(&sums[warp][first + 4]) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+    __syncthreads();
+    if (const int c = threadIdx.x; c < cols) {
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) s += sums[w][c];
+        a.part[(int64_t)blockIdx.x * cols + c] = s;
+    }
+}
+
+/* A block per row, its rows arriving in shared memory by bulk copies `stages` rows ahead: a row is a chain of load, sum over
+ * the block, store, and without the copies a block would have nothing on the way during most of it (8192 x 4096 bf16:
+ * 122 us with loads into registers). */
+template <typename T, int VPT>
+__global__ void __launch_bounds__(512, VPT == 1 ? 2 : 1)
+decxb_rmsnorm_backward_rows_kernel(const NormBwdArgs a, const int stages, const long long wait_limit_ns, decxb_dev_status* status)
+{
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float2 buf[2][16];
+    __shared__ __align__(8) uint64_t bars[8];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nwarps = blockDim.x >> 5, cols = (int)a.cols;
+    const int arrays = a.dr ? 3 : 2;
+    const uint32_t row_bytes = (uint32_t)cols * (uint32_t)sizeof(T);
+    auto first = [&](int i) { return (i * (int)blockDim.x + tid) * 8; };
+    auto fetch = [&](int64_t row, int st) {
+        const uint32_t bar = tcptx::smem_u32(&bars[st]), at = tcptx::smem_u32(smem) + (uint32_t)(st * arrays) * row_bytes;
+        tcptx::mbar_arrive_expect_tx(bar, row_bytes * arrays);
+        bulk_load(at, static_cast<const T*>(a.dy) + row * a.lddy, row_bytes, bar);
+        bulk_load(at + row_bytes, static_cast<const T*>(a.h) + row * a.ldh, row_bytes, bar);
+        if (a.dr) bulk_load(at + 2 * row_bytes, static_cast<const T*>(a.dr) + row * a.lddr, row_bytes, bar);
+    };
+    if (tid == 0) {
+        for (int st = 0; st < stages; ++st) tcptx::mbar_init(tcptx::smem_u32(&bars[st]), 1);
+        tcptx::fence_barrier_init();
+    }
+    __syncthreads();
+    start_after_previous();
+    if (tid == 0)
+        for (int st = 0; st < stages; ++st)
+            if (blockIdx.x + (int64_t)st * gridDim.x < a.rows) fetch(blockIdx.x + (int64_t)st * gridDim.x, st);
+    constexpr bool KEEP = VPT < 4;            /* gamma in registers; with four vectors a thread it is read again every row */
+    float acc[VPT][8], g[KEEP ? VPT : 1][8];
+    auto gamma = [&](int i) -> const float* {
+        if constexpr (KEEP) return g[i];
+        else { load8_any(a.gamma, a.gamma_type, first(i), cols - first(i), true, g[0]); return g[0]; }
+    };
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+        if constexpr (KEEP) load8_any(a.gamma, a.gamma_type, first(i), cols - first(i), true, g[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[i][j] = 0.0f;
+    }
+    int st = 0, turn = 0; uint32_t phase = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+        /* (a copy that does not come within the limit is recorded; the rows that it leaves wrong are the caller's to discard) */
+        wait_copy(tcptx::smem_u32(&bars[st]), phase, wait_limit_ns, status);
+        const T* in = reinterpret_cast<const T*>(smem + (size_t)(st * arrays) * row_bytes);
+        Raw8<T> rw[VPT], rx[VPT], ro[VPT];
+        float sq = 0.0f, dot = 0.0f;
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            const int n = first(i) < cols ? 8 : 0;
+            load_raw(in + first(i), n, true, rw[i]);
+            load_raw(in + cols + first(i), n, true, rx[i]);
+            load_raw(in + 2 * cols + first(i), a.dr ? n : 0, true, ro[i]);
+            float w[8], x[8];
+            unpack(rw[i], w); unpack(rx[i], x);
+            const float* gi = gamma(i);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { sq = fmaf(x[j], x[j], sq); dot = fmaf(w[j] * gi[j], x[j], dot); }
+        }
+        /* behind the barrier in here every thread has its values: the stage can be filled again */
+        const float2 s = block_sum2(sq, dot, buf[turn], warp, lane, nwarps);
+        if (tid == 0 && row + (int64_t)stages * gridDim.x < a.rows) fetch(row + (int64_t)stages * gridDim.x, st);
+        const float r = rsqrtf(s.x / (float)cols + a.eps), k = r * r * (s.y / (float)cols);
+#pragma unroll
+        for (int i = 0; i < VPT; ++i) {
+            float w[8], x[8], o[8];
+            unpack(rw[i], w); unpack(rx[i], x); unpack(ro[i], o);
+            backward8(w, x, gamma(i), r, k, o, acc[i]);
+            if (first(i) < cols) store8(static_cast<T*>(a.dx) + row * a.lddx + first(i), 8, true, o);
+        }
+        if (++st == stages) { st = 0; phase ^= 1u; }
+    }
+    if (!a.part) return;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i)
+        if (first(i) < cols) store8(a.part + (int64_t)blockIdx.x * cols + first(i), 8, true, acc[i]);
+}
+
+/* Rows too long for that, or not aligned for it: each row is read twice and the sums for dgamma live in the workspace. */
 template <typename T>
 __global__ void __launch_bounds__(512)
 decxb_rmsnorm_backward_wide_kernel(const NormBwdArgs a)
 {
     __shared__ float2 buf[2][32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nwarps = blockDim.x >> 5;
+    start_after_previous();
     int turn = 0;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
         const T* dy = static_cast<const T*>(a.dy) + row * a.lddy;
@@ -296,11 +428,12 @@ decxb_rmsnorm_backward_wide_kernel(const NormBwdArgs a)
 
 /* dgamma[c] = sum over the workspace's rows: 32 columns a block, 32 groups of rows side by side. */
 __global__ void __launch_bounds__(1024)
-decxb_column_sum_kernel(const float* __restrict__ part, int parts, int64_t cols, float* __restrict__ out)
+decxb_column_sum_kernel(const float* part, int parts, int64_t cols, float* out)
 {
     __shared__ float sums[32][33];
     const int lane = threadIdx.x & 31, group = threadIdx.x >> 5;
     const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+    start_after_previous();
     float v = 0.0f;
     if (c < cols)
         for (int p = group; p < parts; p += 32) v += part[(int64_t)p * cols + c];
@@ -311,32 +444,45 @@ decxb_column_sum_kernel(const float* __restrict__ part, int parts, int64_t cols,
     if (lane == 0 && co < cols) out[co] = v;
 }
 
-/* Blocks of the backward kernel = rows of its workspace. */
-int64_t backward_blocks(const decxb_ctx* ctx, int64_t rows)
+/* Blocks to an SM, whose sums are the rows of the workspace: more of them where rows are short and a block's chain of load,
+ * sum and store has little to move (16384 x 1024: 2 blocks and a warp a row 101 us). */
+constexpr int64_t WARP_COLS = 256;
+int64_t backward_per_sm(int64_t cols) { return cols <= WARP_COLS ? 4 : cols <= 1024 ? 8 : cols <= 2048 ? 4 : cols <= 8192 ? 2 : 1; }
+int64_t backward_blocks(const decxb_ctx* ctx, int64_t rows, int64_t cols)
 {
-    const int64_t most = (int64_t)ctx->sm_count * 2;
-    return rows < most ? rows : most;
+    const int64_t most = ctx->sm_count * backward_per_sm(cols), have = cols <= WARP_COLS ? decxb_ceil_div(rows, 8) : rows;
+    return have < most ? have : most;
+}
+
+template <typename T, int VPT>
+int launch_backward_rows(decxb_ctx* ctx, const NormBwdArgs& a, unsigned grid, int stages, size_t smem, cudaStream_t s)
+{
+    auto kernel = decxb_rmsnorm_backward_rows_kernel<T, VPT>;
+    static std::once_flag once[DECXB_MAX_DEVICES];
+    static cudaError_t err[DECXB_MAX_DEVICES];
+    std::call_once(once[ctx->device], [&] { err[ctx->device] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024); });
+    if (err[ctx->device] != cudaSuccess) return decxb_fail(ctx, DECXB_ERR_CUDA, std::string("norm kernel attributes: ") + cudaGetErrorString(err[ctx->device]));
+    return launch_after(ctx, kernel, grid, threads_for(decxb_ceil_div(a.cols, 8), VPT, 512), smem, s, a, stages, ctx->wait_limit_ns, ctx->d_status);
 }
 
 template <typename T>
 int launch_norm_backward(decxb_ctx* ctx, const NormBwdArgs& a, float* dgamma, cudaStream_t s)
 {
-    const int64_t nvec = decxb_ceil_div(a.cols, 8);
-    const unsigned grid = (unsigned)backward_blocks(ctx, a.rows);
-    {
-        decxb_launch_scope scope(ctx, s, DECXB_K_SPLIT);
-        if (nvec <= 512)       decxb_rmsnorm_backward_kernel<T, 1><<<grid, threads_for(nvec, 1, 512), 0, s>>>(a);
-        else if (nvec <= 1024) decxb_rmsnorm_backward_kernel<T, 2><<<grid, threads_for(nvec, 2, 512), 0, s>>>(a);
-        else if (nvec <= 2048) decxb_rmsnorm_backward_kernel<T, 4><<<grid, threads_for(nvec, 4, 512), 0, s>>>(a);
-        else                   decxb_rmsnorm_backward_wide_kernel<T><<<grid, 512, 0, s>>>(a);
-        DECXB_CUDA_TRY(ctx, cudaGetLastError());
-    }
-    if (dgamma) {
-        decxb_launch_scope scope(ctx, s, DECXB_K_SPLIT);
-        decxb_column_sum_kernel<<<(unsigned)decxb_ceil_div(a.cols, 32), 1024, 0, s>>>(a.part, (int)grid, a.cols, dgamma);
-        DECXB_CUDA_TRY(ctx, cudaGetLastError());
-    }
-    return DECXB_OK;
+    const int64_t nvec = decxb_ceil_div(a.cols, 8), grid = backward_blocks(ctx, a.rows, a.cols);
+    const int64_t row_bytes = a.cols * (int64_t)sizeof(T) * (a.dr ? 3 : 2);
+    int64_t stages = 220 * 1024 / backward_per_sm(a.cols) / row_bytes;       /* rows of a block in shared memory */
+    if (stages > 4) stages = 4;
+    int rc;
+    if (a.cols <= WARP_COLS) rc = launch_after(ctx, decxb_rmsnorm_backward_kernel<T>, (unsigned)grid, 256, 0, s, a);
+    else if (a.vec && a.gvec && a.cols % 8 == 0 && nvec <= 2048 && stages >= 2)
+        rc = nvec <= 512  ? launch_backward_rows<T, 1>(ctx, a, (unsigned)grid, (int)stages, (size_t)(stages * row_bytes), s)
+           : nvec <= 1024 ? launch_backward_rows<T, 2>(ctx, a, (unsigned)grid, (int)stages, (size_t)(stages * row_bytes), s)
+                          : launch_backward_rows<T, 4>(ctx, a, (unsigned)grid, (int)stages, (size_t)(stages * row_bytes), s);
+    else
+        rc = launch_after(ctx, decxb_rmsnorm_backward_wide_kernel<T>, (unsigned)grid, 512, 0, s, a);
+    if (rc == DECXB_OK && dgamma)
+        rc = launch_after(ctx, decxb_column_sum_kernel, (unsigned)decxb_ceil_div(a.cols, 32), 1024, 0, s, (const float*)a.part, (int)grid, a.cols, dgamma);
+    return rc;
 }
 
 /* ---- quantisation -------------------------------------------------------------------------
@@ -371,8 +517,8 @@ __device__ __forceinline__ uint32_t shuffle_max(uint32_t a, int o)
     return max_word(a, __shfl_xor_sync(0xffffffffu, a, o), static_cast<const T*>(nullptr));
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2)
+template <typename T, int TYPE>
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2)
 decxb_quantize_fp8_kernel(const QuantArgs a)
 {
     /* W words hold the eight columns of a row, E columns to a word; magnitudes are compared as words, two columns of 16 bits at once */
@@ -381,6 +527,7 @@ decxb_quantize_fp8_kernel(const QuantArgs a)
     const T* const kind = nullptr;
     __shared__ uint32_t colmax[8][16 * W];
     __shared__ uint32_t wmax[8];
+    __shared__ float colscale[128];
     __shared__ __align__(16) uint8_t tr[128 * 128];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = tid >> 4, t = tid & 15;
     const int64_t tile_r = blockIdx.x / a.tiles_c, tile_c = blockIdx.x % a.tiles_c;
@@ -388,6 +535,7 @@ decxb_quantize_fp8_kernel(const QuantArgs a)
     const int64_t row = r0 + g * 8, col = c0 + t * 8;
     const int nr = (int)max((int64_t)0, min((int64_t)8, a.rows - row));          /* rows and columns that exist here */
     const int nc = (int)max((int64_t)0, min((int64_t)8, a.cols - col));
+    start_after_previous();
     Raw8<T> x[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) load_raw(static_cast<const T*>(a.x) + (row + i) * a.ldx + col, i < nr ? nc : 0, a.vec, x[i]);
@@ -424,53 +572,71 @@ decxb_quantize_fp8_kernel(const QuantArgs a)
         for (int e = 0; e < E; ++e) tile_max = max_nan(tile_max, lane_of(m, e));
     }
 
-    if (a.q.data) {
-        const float st = a.q.block_rows == 128 ? scale_of(tile_max, a.q.type, a.rule) : 0.0f;
-        if (a.q.block_rows == 128 && tid == 0) a.q.s[tile_r * a.q.srs + tile_c * a.q.sbs] = st;
+    /* one thread a column makes the scales of the transpose's rows while the others go on */
+    if (by_col && tid < 128) {
+        uint32_t m = colmax[0][tid / E];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float s = st;
-            if (a.q.block_rows == 1) {
+        for (int w = 1; w < 8; ++w) m = max_word(m, colmax[w][tid / E], kind);
+        const float s = scale_of(lane_of(m, tid % E), TYPE, a.rule);
+        if (c0 + tid < a.cols) a.t.s[(c0 + tid) * a.t.srs + tile_r * a.t.sbs] = s;
+        colscale[tid] = s;
+    }
+
+    if (a.q.data) {
+        float s = 0.0f;
+        if (a.q.block_rows == 128) {
+            s = scale_of(tile_max, TYPE, a.rule);
+            if (tid == 0) a.q.s[tile_r * a.q.srs + tile_c * a.q.sbs] = s;
+        } else {
+            /* largest of each of the eight rows, halved over the lanes at every exchange: lane t ends with row t / 2 */
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
                 uint32_t m = word(i, 0) & MAG;
 #pragma unroll
                 for (int k = 1; k < W; ++k) m = max_word(m, word(i, k) & MAG, kind);
-                float f = lane_of(m, 0);
-                if (E == 2) f = max_nan(f, lane_of(m, E - 1));
+                f[i] = lane_of(m, 0);
+                if (E == 2) f[i] = max_nan(f[i], lane_of(m, E - 1));
+            }
 #pragma unroll
-                for (int o = 8; o; o >>= 1) f = max_nan(f, __shfl_xor_sync(0xffffffffu, f, o));
-                s = scale_of(f, a.q.type, a.rule);
-                if (t == 0 && i < nr) a.q.s[(row + i) * a.q.srs + tile_c * a.q.sbs] = s;
+            for (int n = 4; n; n >>= 1) {
+                const bool up = t & (2 * n);
+#pragma unroll
+                for (int i = 0; i < n; ++i) {
+                    const float keep = up ? f[n + i] : f[i], give = up ? f[i] : f[n + i];
+                    f[i] = max_nan(keep, __shfl_xor_sync(0xffffffffu, give, 2 * n));
+                }
+            }
+            f[0] = max_nan(f[0], __shfl_xor_sync(0xffffffffu, f[0], 1));
+            s = scale_of(f[0], TYPE, a.rule);
+            if ((t & 1) == 0 && (t >> 1) < nr) a.q.s[(row + (t >> 1)) * a.q.srs + tile_c * a.q.sbs] = s;
+        }
+        Quantiser z = quantiser(s);
+        const float s_row = z.s, inv_row = z.inv;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (a.q.block_rows == 1) {
+                z.s = __shfl_sync(0xffffffffu, s_row, 2 * i, 16);
+                z.inv = __shfl_sync(0xffffffffu, inv_row, 2 * i, 16);
             }
             float v[8];
             unpack(x[i], v);
-            if (i < nr && nc > 0) store_codes8(a.q.data + (row + i) * a.q.ld + col, nc, a.q.vec, codes8(v, quantiser(s, a.rule), a.q.type));
+            if (i < nr && nc > 0) store_codes8(a.q.data + (row + i) * a.q.ld + col, nc, a.q.vec, codes8<TYPE>(v, z));
         }
     }
 
     if (a.t.data) {
-        const float st = a.t.block_rows == 128 ? scale_of(tile_max, a.t.type, a.rule) : 0.0f;
+        if (by_col) __syncthreads();
+        const float st = a.t.block_rows == 128 ? scale_of(tile_max, TYPE, a.rule) : 0.0f;
         if (a.t.block_rows == 128 && tid == 0) a.t.s[tile_c * a.t.srs + tile_r * a.t.sbs] = st;
+        Quantiser z = quantiser(st);
 #pragma unroll
-        for (int k = 0; k < W; ++k) {
-            uint32_t m = 0;
-            if (by_col) {
-                m = colmax[0][t * W + k];
+        for (int j = 0; j < 8; ++j) {
+            if (by_col) z = quantiser(colscale[t * 8 + j]);
+            float v[8];
 #pragma unroll
-                for (int w = 1; w < 8; ++w) m = max_word(m, colmax[w][t * W + k], kind);
-            }
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int j = k * E + e;
-                float s = st;
-                if (by_col) {
-                    s = scale_of(lane_of(m, e), a.t.type, a.rule);
-                    if (g == 0 && j < nc) a.t.s[(col + j) * a.t.srs + tile_r * a.t.sbs] = s;
-                }
-                float v[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = lane_of(word(i, k), e);
-                *reinterpret_cast<uint2*>(tr + (t * 8 + j) * 128 + ((g ^ t) << 3)) = codes8(v, quantiser(s, a.rule), a.t.type);
-            }
+            for (int i = 0; i < 8; ++i) v[i] = lane_of(word(i, j / E), j % E);
+            *reinterpret_cast<uint2*>(tr + (t * 8 + j) * 128 + ((g ^ t) << 3)) = codes8<TYPE>(v, z);
         }
         __syncthreads();
         /* out: row c of the transpose, eight of X's rows per thread, 16 lanes a row */
@@ -489,10 +655,9 @@ int launch_quantize(decxb_ctx* ctx, const QuantArgs& a, cudaStream_t s)
 {
     const int64_t tiles = decxb_ceil_div(a.rows, 128) * a.tiles_c;
     if (tiles > 0x7fffffffLL) return decxb_fail(ctx, DECXB_ERR_TOO_LARGE, "tiles of 128 x 128");
-    decxb_launch_scope scope(ctx, s, DECXB_K_SPLIT);
-    decxb_quantize_fp8_kernel<T><<<(unsigned)tiles, 256, 0, s>>>(a);
-    DECXB_CUDA_TRY(ctx, cudaGetLastError());
-    return DECXB_OK;
+    return (a.q.data ? a.q.type : a.t.type) == DECXB_FP8_E4M3
+        ? launch_after(ctx, decxb_quantize_fp8_kernel<T, DECXB_FP8_E4M3>, (unsigned)tiles, 256, 0, s, a)
+        : launch_after(ctx, decxb_quantize_fp8_kernel<T, DECXB_FP8_E5M2>, (unsigned)tiles, 256, 0, s, a);
 }
 
 QuantArgs::Out out_of(const decxb_fp8_matrix* m)
@@ -514,6 +679,10 @@ int quantize(decxb_ctx* ctx, int x_type, int64_t rows, int64_t cols, const void*
     if (Qt && (rc = check_output(ctx, Qt, "Qt", cols, rows))) return rc;
     if (rows == 0 || cols == 0) return DECXB_OK;
     if ((rc = check_array(ctx, X, ldx, cols, size_of(x_type), "X"))) return rc;
+    if (Q && Qt && Q->type != Qt->type) {         /* one type a launch */
+        rc = quantize(ctx, x_type, rows, cols, X, ldx, rule, Q, nullptr, s);
+        return rc ? rc : quantize(ctx, x_type, rows, cols, X, ldx, rule, nullptr, Qt, s);
+    }
     QuantArgs a = {};
     a.rows = rows; a.cols = cols; a.x = X; a.ldx = ldx; a.rule = rule;
     a.vec = aligned(X, ldx * size_of(x_type), 16);
@@ -568,7 +737,7 @@ int norm(decxb_ctx* ctx, int type, int64_t rows, int64_t cols, const void* X, in
 
 size_t backward_bytes(const decxb_ctx* ctx, int64_t rows, int64_t cols)
 {
-    return (size_t)backward_blocks(ctx, rows) * (size_t)cols * sizeof(float);
+    return (size_t)backward_blocks(ctx, rows, cols) * (size_t)cols * sizeof(float);
 }
 
 int norm_backward(decxb_ctx* ctx, int type, int64_t rows, int64_t cols, const void* dY, int64_t lddy, const void* H, int64_t ldh,

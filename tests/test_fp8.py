@@ -304,6 +304,18 @@ def test_quantise_strides_and_one_output(ctx, pad, offset):
 
 
 @gpu
+def test_quantise_orientations_of_different_types(ctx):
+    x = torch.randn(200, 300, device=DEV)
+    Q, T = b.Fp8Matrix.empty(200, 300, 1, b.FP8_E4M3), b.Fp8Matrix.empty(300, 200, 128, b.FP8_E5M2)
+    ctx.quantize_fp8(200, 300, x, 300, Q, T, stream=cur())
+    ctx.synchronize()
+    for m, y, blk, kind in ((Q, x.double(), 1, b.FP8_E4M3), (T, x.double().t(), 128, b.FP8_E5M2)):
+        s = want_scales(blocks_amax(y, blk), kind, b.SCALE_AMAX)
+        assert torch.equal(m.scales, s)
+        check_codes(m.data, y / spread(s, blk, *y.shape).double(), kind, 0.0)
+
+
+@gpu
 def test_quantise_zeros_nan_infinity_and_tiny(ctx):
     x = torch.randn(6, 256, device=DEV)
     x[0] = 0.0
@@ -559,7 +571,7 @@ def test_norm_refusals(ctx):
         assert e.value.status == status, str(e.value)
 
     ws = torch.empty(8192, device=DEV, dtype=torch.uint8)
-    badb(13, workspace=ws, workspace_bytes=4 * 256 * 4 - 1)
+    badb(13, workspace=ws, workspace_bytes=ctx.rmsnorm_backward_workspace(4, 256) - 1)
     badb(13, workspace=ws[4:], workspace_bytes=8000)
     badb(13, dX=x)
     badb(3, lddx=255)
