@@ -190,13 +190,21 @@ _DTYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16,
 _FP8_TYPES = {"torch.float8_e4m3fn": FP8_E4M3, "torch.float8_e5m2": FP8_E5M2}
 
 
+_known_dtypes = {}      # element type objects already looked up by name
+
+
 def _dtype(x, given):
     """F32 / F16 / BF16 of an array argument; `given` (needed for raw addresses) has to agree with a tensor's own."""
-    own = _DTYPES.get(str(getattr(x, "dtype", "")))
+    dt = getattr(x, "dtype", None)
+    own = _known_dtypes.get(dt)
+    if own is None and dt is not None:
+        own = _DTYPES.get(str(dt))
+        if own is not None:
+            _known_dtypes[dt] = own
     if own is None and given is None:
-        raise TypeError(f"element type of {type(x).__name__} {getattr(x, 'dtype', '')} is not F32, F16 or BF16: pass it")
+        raise TypeError(f"element type of {type(x).__name__} {dt} is not F32, F16 or BF16: pass it")
     if own is not None and given is not None and own != given:
-        raise TypeError(f"element type {given} given for an array of {x.dtype}")
+        raise TypeError(f"element type {given} given for an array of {dt}")
     return own if given is None else given
 
 
@@ -217,7 +225,7 @@ class Fp8Matrix:
         self.c = Fp8MatrixStruct(_ptr(data), _ptr(scales), rows, cols, ld, scale_row_stride, scale_block_stride, type, block_rows)
         self.addr = C.addressof(self.c)
         self.rows, self.cols, self.block_rows, self.type = rows, cols, block_rows, type
-        self.tensors = tuple(t for t in (data, scales) if hasattr(t, "is_cuda"))
+        self.devices = tuple(t.get_device() for t in (data, scales) if hasattr(t, "get_device"))
 
     @classmethod
     def of(cls, data, scales, block_rows=1):
@@ -379,37 +387,58 @@ class Context:
         self._chk(self.L.decxb_gemm_release_b(self.h, pb, stream))
 
     # -- 8-bit linear layer -----------------------------------------------------------------
-    def _here(self, *args):
-        """Tensor arguments have to lie on the context's device (a raw address is the caller's word)."""
-        for a in args:
-            for t in a.tensors if isinstance(a, Fp8Matrix) else (a,):
-                if hasattr(t, "is_cuda") and not (t.is_cuda and t.device.index == self.device):
-                    raise DecxbError(13, f"a tensor on {t.device} was passed to a context of cuda:{self.device}")
+    def _at(self, x):
+        """Address of an array argument; a tensor has to lie on the context's device (a raw address is the caller's word)."""
+        if x is None:
+            return None
+        try:
+            on = x.get_device()
+        except AttributeError:
+            return _ptr(x)
+        if on != self.device:
+            raise DecxbError(13, f"a tensor on {x.device} was passed to a context of cuda:{self.device}")
+        return x.data_ptr()
+
+    def _fp8(self, m):
+        """Address of an fp8 matrix argument's descriptor."""
+        if m is None:
+            return None
+        for on in m.devices:
+            if on != self.device:
+                raise DecxbError(13, f"an fp8 matrix on device {on} was passed to a context of cuda:{self.device}")
+        return m.addr
+
+    def _on(self, stream, some_tensor):
+        """Handle of a `stream` argument.  Without one the work runs on the context's own stream, after what torch has queued."""
+        if stream is None and getattr(some_tensor, "is_cuda", False):
+            import torch
+
+            torch.cuda.current_stream(some_tensor.device).synchronize()
+        return _stream(stream)
 
     def gemm_fp8(self, A: Fp8Matrix, B: Fp8Matrix, D, ldd, Cin=None, ldc=0, d_type=None, stream=None):
         """D[A.rows][B.rows] = A B^T (+ Cin), both operands K-contiguous with their block scales (decxb_gemm_fp8)."""
-        self._here(A, B, D, Cin)
         t = _dtype(D, d_type)
         if Cin is not None:
             _dtype(Cin, t)
-        self._chk(self.L.decxb_gemm_fp8(self.h, A.addr, B.addr, _ptr(Cin), ldc, _ptr(D), t, ldd, _stream(stream)))
+        self._chk(self.L.decxb_gemm_fp8(self.h, self._fp8(A), self._fp8(B), self._at(Cin), ldc, self._at(D), t, ldd,
+                                        self._on(stream, A.data)))
 
     def quantize_fp8(self, rows, cols, X, ldx, Q: Fp8Matrix = None, Qt: Fp8Matrix = None, rule=SCALE_AMAX, x_type=None, stream=None):
         """X [rows][cols] into Q and / or, transposed, into Qt (decxb_quantize_fp8)."""
-        self._here(X, Q, Qt)
-        self._chk(self.L.decxb_quantize_fp8(self.h, _dtype(X, x_type), rows, cols, _ptr(X), ldx, rule,
-                                            Q.addr if Q else None, Qt.addr if Qt else None, _stream(stream)))
+        self._chk(self.L.decxb_quantize_fp8(self.h, _dtype(X, x_type), rows, cols, self._at(X), ldx, rule, self._fp8(Q), self._fp8(Qt),
+                                            self._on(stream, X)))
 
     def rmsnorm(self, rows, cols, X, ldx, gamma, eps, R=None, ldr=0, H=None, ldh=0, Y=None, ldy=0, Q: Fp8Matrix = None,
                 rule=SCALE_AMAX, type=None, gamma_type=None, stream=None):
         """h = X (+ R), y = h / rms(h) * gamma into H, Y and, quantised, Q, whichever are given (decxb_rmsnorm)."""
-        self._here(X, gamma, R, H, Y, Q)
         t = _dtype(X, type)
         for a in (R, H, Y):
             if a is not None:
                 _dtype(a, t)
-        self._chk(self.L.decxb_rmsnorm(self.h, t, rows, cols, _ptr(X), ldx, _ptr(R), ldr, _ptr(gamma), _dtype(gamma, gamma_type),
-                                       eps, _ptr(H), ldh, _ptr(Y), ldy, rule, Q.addr if Q else None, _stream(stream)))
+        self._chk(self.L.decxb_rmsnorm(self.h, t, rows, cols, self._at(X), ldx, self._at(R), ldr, self._at(gamma),
+                                       _dtype(gamma, gamma_type), eps, self._at(H), ldh, self._at(Y), ldy, rule, self._fp8(Q),
+                                       self._on(stream, X)))
 
     def rmsnorm_backward_workspace(self, rows, cols) -> int:
         n = _sz()
@@ -419,16 +448,15 @@ class Context:
     def rmsnorm_backward(self, rows, cols, dY, lddy, H, ldh, gamma, eps, dX, lddx, dgamma=None, dR=None, lddr=0,
                          workspace=None, workspace_bytes=0, type=None, gamma_type=None, stream=None):
         """Gradients of rmsnorm's y: dX (with dR added) and dgamma, fp32 (decxb_rmsnorm_backward)."""
-        self._here(dY, H, gamma, dX, dgamma, dR, workspace)
         t = _dtype(H, type)
         for a in (dY, dX, dR):
             if a is not None:
                 _dtype(a, t)
         if dgamma is not None:
             _dtype(dgamma, F32)
-        self._chk(self.L.decxb_rmsnorm_backward(self.h, t, rows, cols, _ptr(dY), lddy, _ptr(H), ldh, _ptr(gamma),
-                                                _dtype(gamma, gamma_type), eps, _ptr(dR), lddr, _ptr(dX), lddx, _ptr(dgamma),
-                                                _ptr(workspace), workspace_bytes, _stream(stream)))
+        self._chk(self.L.decxb_rmsnorm_backward(self.h, t, rows, cols, self._at(dY), lddy, self._at(H), ldh, self._at(gamma),
+                                                _dtype(gamma, gamma_type), eps, self._at(dR), lddr, self._at(dX), lddx, self._at(dgamma),
+                                                self._at(workspace), workspace_bytes, self._on(stream, gamma)))
 
     # -- convolution ----------------------------------------------------------------------
     def set_pack_variant(self, variant: int):
@@ -497,7 +525,6 @@ def _order_after_torch(fn):
     def wrapper(self, *args, **kwargs):
         if kwargs.get("stream") is None:
             for a in list(args) + list(kwargs.values()):
-                a = a.data if isinstance(a, Fp8Matrix) else a
                 if getattr(a, "is_cuda", False):
                     import torch
 
@@ -509,7 +536,7 @@ def _order_after_torch(fn):
 
 for _name in ("fill_uniform", "gemm", "gemm_act", "gemm_nt", "gemm_f16", "gemm_batched", "prepare_b", "gemm_prepared",
               "im2col_pack", "conv2_im2col", "conv2_im2col_act", "conv2_im2col_prepared", "conv_prepare_filters",
-              "gemm_rowshard", "conv2_im2col_batchshard", "gemm_fp8", "quantize_fp8", "rmsnorm", "rmsnorm_backward"):
+              "gemm_rowshard", "conv2_im2col_batchshard"):
     setattr(Context, _name, _order_after_torch(getattr(Context, _name)))
 
 
