@@ -54,7 +54,7 @@ struct Params {
     const void* C; int64_t ldc;
     void* D; int64_t ldd;
     int d_type;
-    bool tma_store;                /* D leaves through the copy engine                 */
+    bool tma_store;                /* D leaves, and C comes, through the copy engine   */
     bool d_vec;                    /* four results of a row may leave in one store      */
     long long wait_limit_ns;
     decxb_dev_status* status;
@@ -194,24 +194,26 @@ __device__ __forceinline__ void tile_coords(int t, int tiles_m, int tiles_n, int
  * stores would touch 32 rows an instruction (8000 clocks for a warp's 128 columns, a sixth of a K = 8192 tile).
  * 16-byte pieces are XOR-ed with the row, which is the copy engine's 128-byte swizzle and keeps the banks apart.
  *
- * Through the copy engine: `n` 16-byte pieces of this row (8 of them fill the box), then one store of the box. */
-template <typename T>
+ * Through the copy engine: 16-byte pieces of this row from `first` on (8 of them fill the box), then one store of the box.
+ * ADD: the box holds the addend, brought there by the copy engine before. */
+template <typename T, bool ADD>
 __device__ __forceinline__ void box_pieces(uint32_t box, int lane, int first, const float* v)
 {
     constexpr int E = 16 / sizeof(T);
 #pragma unroll
     for (int j = 0; j < 32; j += E) {
+        const uint32_t at = box + (uint32_t)lane * 128u + (uint32_t)(((first + j / E) ^ (lane & 7)) << 4);
         uint4 u;
         T* e = reinterpret_cast<T*>(&u);
+        if (ADD) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(at) : "memory");
 #pragma unroll
-        for (int k = 0; k < E; ++k) e[k] = from_f32<T>(v[j + k]);
-        const uint32_t at = box + (uint32_t)lane * 128u + (uint32_t)(((first + j / E) ^ (lane & 7)) << 4);
+        for (int k = 0; k < E; ++k) e[k] = from_f32<T>(ADD ? v[j + k] + to_f32(e[k]) : v[j + k]);
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" :: "r"(at), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
     }
 }
 
 /* The same from registers in the 16x256b shape (two lane halves of four groups of eight columns). */
-template <typename T>
+template <typename T, bool ADD>
 __device__ __forceinline__ void box_fragments(uint32_t box, int lane, int first, const float* v)
 {
 #pragma unroll
@@ -220,19 +222,32 @@ __device__ __forceinline__ void box_fragments(uint32_t box, int lane, int first,
         const uint32_t row = box + (uint32_t)r * 128u;
         if constexpr (sizeof(T) == 4) {
             const uint32_t at = row + (uint32_t)(((2 * g + ((lane & 3) >> 1)) ^ (r & 7)) << 4) + (uint32_t)(lane & 1) * 8u;
-            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" :: "r"(at), "f"(v[i]), "f"(v[i + 1]) : "memory");
+            float2 c = make_float2(0.0f, 0.0f);
+            if (ADD) c = lds_f32x2(at);
+            asm volatile("st.shared.v2.f32 [%0], {%1, %2};" :: "r"(at), "f"(v[i] + c.x), "f"(v[i + 1] + c.y) : "memory");
         } else {
-            alignas(4) T e[2] = {from_f32<T>(v[i]), from_f32<T>(v[i + 1])};
             const uint32_t at = row + (uint32_t)(((first + g) ^ (r & 7)) << 4) + (uint32_t)(lane & 3) * 4u;
-            asm volatile("st.shared.b32 [%0], %1;" :: "r"(at), "r"(*reinterpret_cast<const uint32_t*>(e)) : "memory");
+            uint32_t u = 0;
+            if (ADD) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(u) : "r"(at) : "memory");
+            T* e = reinterpret_cast<T*>(&u);
+            e[0] = from_f32<T>(ADD ? v[i] + to_f32(e[0]) : v[i]);
+            e[1] = from_f32<T>(ADD ? v[i + 1] + to_f32(e[1]) : v[i + 1]);
+            asm volatile("st.shared.b32 [%0], %1;" :: "r"(at), "r"(u) : "memory");
         }
     }
 }
-template <typename T, bool FRAGMENTS>
-__device__ __forceinline__ void box_write(uint32_t box, int lane, int first, const float* v)
+template <bool FRAGMENTS, bool ADD>
+__device__ __forceinline__ void box_write(int type, uint32_t box, int lane, int first, const float* v)
 {
-    if constexpr (FRAGMENTS) box_fragments<T>(box, lane, first, v);
-    else                     box_pieces<T>(box, lane, first, v);
+    if constexpr (FRAGMENTS) {
+        if (type == DECXB_F32)      box_fragments<float, ADD>(box, lane, first, v);
+        else if (type == DECXB_F16) box_fragments<__half, ADD>(box, lane, first, v);
+        else                        box_fragments<__nv_bfloat16, ADD>(box, lane, first, v);
+    } else {
+        if (type == DECXB_F32)      box_pieces<float, ADD>(box, lane, first, v);
+        else if (type == DECXB_F16) box_pieces<__half, ADD>(box, lane, first, v);
+        else                        box_pieces<__nv_bfloat16, ADD>(box, lane, first, v);
+    }
 }
 
 /* By the threads, row after row with one column a lane: any address and pitch, and the addend on the way. */
@@ -278,6 +293,8 @@ __device__ __forceinline__ void put4(const Params& p, int64_t row, int64_t col, 
  * Many result tiles: a pair of CTAs (cta_group::2) per tile of 256 x 256, each with 128 rows of A and 128 of B.
  * COLVEC : B has a scale per row (block_rows 1): each column of the tile has its own factor.  Otherwise a
  *          128-row block of B has one scale, and the columns of one epilogue warp lie in one block.
+ * ADDEND : C comes through the copy engine into the boxes that the results leave from, the first of a tile during its
+ *          product (4096 x 4096 x 8192 with an fp32 addend: 436 us with the threads' own loads).
  * ------------------------------------------------------------------------------------ */
 template <bool COLVEC>
 struct Cfg {
@@ -301,10 +318,10 @@ struct Cfg {
     static_assert(STAGES > BUFS, "a stage's barrier must not turn over twice unseen");
 };
 
-template <bool COLVEC>
+template <bool COLVEC, bool ADDEND>
 __global__ void __launch_bounds__(THREADS, 1)
 decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                      const __grid_constant__ CUtensorMap map_d, const Params p)
+                      const __grid_constant__ CUtensorMap map_d, const __grid_constant__ CUtensorMap map_c, const Params p)
 {
     using C = Cfg<COLVEC>;
     extern __shared__ uint8_t smem_raw[];
@@ -317,7 +334,8 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     auto tempty_bar = [&](int b) { return bars + 8u * (2 * C::STAGES + b); };
     auto sfull_bar  = [&](int s) { return bars + 8u * (2 * C::STAGES + C::BUFS + s); };
     auto sempty_bar = [&](int s) { return bars + 8u * (2 * C::STAGES + C::BUFS + SLOTS + s); };
-    const uint32_t tmem_slot = bars + 8u * (2 * C::STAGES + C::BUFS + 2 * SLOTS);
+    auto addend_bar = [&](int w) { return bars + 8u * (2 * C::STAGES + C::BUFS + 2 * SLOTS + w); };
+    const uint32_t tmem_slot = bars + 8u * (2 * C::STAGES + C::BUFS + 2 * SLOTS + EPI_WARPS);
     auto stage_a = [&](int s) { return smem_base + s * C::STAGE_BYTES; };
     auto stage_b = [&](int s) { return smem_base + s * C::STAGE_BYTES + C::A_BYTES; };
 
@@ -330,9 +348,11 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     if (threadIdx.x == 0) {
         prefetch_tensormap(&map_a); prefetch_tensormap(&map_b);
         if (p.tma_store) prefetch_tensormap(&map_d);
+        if (ADDEND) prefetch_tensormap(&map_c);
         for (int s = 0; s < C::STAGES; ++s) { mbar_init(full_bar(s), 1); mbar_init(done_bar(s), 1); }
         for (int b = 0; b < C::BUFS; ++b) mbar_init(tempty_bar(b), EPI_WARPS * C::CTAS);
         for (int s = 0; s < SLOTS; ++s) { mbar_init(sfull_bar(s), 32); mbar_init(sempty_bar(s), EPI_WARPS); }
+        for (int w = 0; w < EPI_WARPS; ++w) mbar_init(addend_bar(w), 1);
         fence_barrier_init();
     }
     if (warp == 1) {
@@ -451,12 +471,26 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int q = warp & 3, eh = (warp - 4) >> 2;
         const uint32_t tlane = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(eh * C::ACC);
-        const uint32_t box = boxes + (uint32_t)(warp - 4) * 4096u;
+        const uint32_t box = boxes + (uint32_t)(warp - 4) * 4096u, cbar = addend_bar(warp - 4);
+        uint32_t cphase = 0;
+        bool pending = false;
+        /* the addend of one box, once the copy engine has read the result that the box held */
+        auto fetch_addend = [&](int64_t col, int64_t row) {
+            tma_store_wait_read<0>();
+            mbar_arrive_expect_tx(cbar, 4096);
+            tma_load_2d(box, &map_c, cbar, (int)col, (int)row);
+        };
         int unit = 0, slot = 0, stage = 0;
         uint32_t sphase = 0, phase = 0;
         bool alive = true;
         for (int t = cluster_id; t < num_tiles && alive; t += num_clusters) {
             int tm, tn; tile_coords(t, p.tiles_m, p.tiles_n, p.tile_group, tm, tn);
+            const int64_t row0 = (int64_t)tm * C::UMMA_M + cta_rank * BM_CTA + q * 32;
+            const int64_t col0 = (int64_t)tn * C::UMMA_N + eh * C::ACC;
+            if (ADDEND && row0 < p.M && col0 < p.N) {
+                if (lane == 0) fetch_addend(col0, row0);
+                pending = true;
+            }
             float sum[C::ACC];
 #pragma unroll
             for (int c = 0; c < C::ACC; ++c) sum[c] = 0.0f;
@@ -517,9 +551,8 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                 if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
             }
             if (!alive) break;
-            const int64_t row0 = (int64_t)tm * C::UMMA_M + cta_rank * BM_CTA + q * 32;
-            const int64_t col0 = (int64_t)tn * C::UMMA_N + eh * C::ACC;
             if (row0 >= p.M) continue;
+            pending = false;
 #pragma unroll
             for (int c = 0; c < C::ACC; c += 32) {
                 if (col0 + c >= p.N) break;
@@ -528,12 +561,16 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                 if (p.tma_store) {
                     const int first = narrow && (c & 32) ? 4 : 0;
                     if (first == 0) {
-                        if (lane == 0) tma_store_wait_read<0>();      /* the box before has been read */
-                        __syncwarp();
+                        if constexpr (ADDEND) {
+                            if (c > 0 && lane == 0) fetch_addend(col0 + c, row0);       /* the first one came during the product */
+                            if (!warp_wait(cbar, cphase, p, 1700 + warp, t)) { alive = false; break; }
+                            cphase ^= 1u;
+                        } else {
+                            if (lane == 0) tma_store_wait_read<0>();      /* the box before has been read */
+                            __syncwarp();
+                        }
                     }
-                    if (!narrow)                        box_write<float, COLVEC>(box, lane, 0, v);
-                    else if (p.d_type == DECXB_F16)     box_write<__half, COLVEC>(box, lane, first, v);
-                    else                                box_write<__nv_bfloat16, COLVEC>(box, lane, first, v);
+                    box_write<COLVEC, ADDEND>(p.d_type, box, lane, first, v);
                     if (!narrow || first || col0 + c + 32 >= p.N) {
                         fence_proxy_async_smem();
                         __syncwarp();
@@ -544,7 +581,7 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                     }
                 } else {
                     __syncwarp();
-                    box_write<float, COLVEC>(box, lane, 0, v);
+                    box_write<COLVEC, false>(DECXB_F32, box, lane, 0, v);
                     __syncwarp();
                     if (!narrow)                        box_rows<float>(p, box, lane, row0, col0 + c + lane);
                     else if (p.d_type == DECXB_F16)     box_rows<__half>(p, box, lane, row0, col0 + c + lane);
@@ -552,6 +589,8 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                 }
             }
         }
+        if (ADDEND && pending && lane == 0)                                 /* a wait gave up: the addend may still be on its way */
+            for (int tries = 0; tries < 2048 && !mbar_try_wait(cbar, cphase); ++tries) __nanosleep(64);
         if (p.tma_store && lane == 0) tma_store_wait_all();       /* the box stays until the copy engine is done */
     }
 
@@ -820,11 +859,11 @@ int make_map_fp8(decxb_ctx* ctx, CUtensorMap* map, const decxb_fp8_matrix& m, in
     return make_map_2d(ctx, map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, m.data, m.rows, m.cols, m.ld, box_rows);
 }
 
-template <bool COLVEC>
+template <bool COLVEC, bool ADDEND>
 int launch(decxb_ctx* ctx, const decxb_fp8_matrix& A, const decxb_fp8_matrix& B, Params p, cudaStream_t s)
 {
     using C = Cfg<COLVEC>;
-    auto kernel = decxb_gemm_fp8_kernel<COLVEC>;
+    auto kernel = decxb_gemm_fp8_kernel<COLVEC, ADDEND>;
     static std::once_flag once[DECXB_MAX_DEVICES];
     static cudaError_t attr_err[DECXB_MAX_DEVICES];
     static int regs[DECXB_MAX_DEVICES];
@@ -841,12 +880,13 @@ int launch(decxb_ctx* ctx, const decxb_fp8_matrix& A, const decxb_fp8_matrix& B,
     CUtensorMap ma, mb;
     int rc;
     if ((rc = make_map_fp8(ctx, &ma, A, BM_CTA)) || (rc = make_map_fp8(ctx, &mb, B, C::BN))) return rc;
-    CUtensorMap md = ma;
+    CUtensorMap md = ma, mc = ma;
     if (p.tma_store) {
         const int e = size_of(p.d_type);
         const CUtensorMapDataType type = p.d_type == DECXB_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                        : p.d_type == DECXB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
         if ((rc = make_map_2d(ctx, &md, type, e, p.D, p.M, p.N, p.ldd, 32))) return rc;
+        if (ADDEND && (rc = make_map_2d(ctx, &mc, type, e, p.C, p.M, p.N, p.ldc, 32))) return rc;
     }
     const int64_t tm = decxb_ceil_div(p.M, C::UMMA_M), tn = decxb_ceil_div(p.N, C::UMMA_N);
     if (tm * tn > 0x7fffffffLL) return decxb_fail(ctx, DECXB_ERR_TOO_LARGE, "fp8 gemm tiles");
@@ -867,7 +907,7 @@ int launch(decxb_ctx* ctx, const decxb_fp8_matrix& A, const decxb_fp8_matrix& B,
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr; cfg.numAttrs = 2;
     decxb_launch_scope scope(ctx, s, DECXB_K_GEMM);
-    DECXB_CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, kernel, ma, mb, md, p));
+    DECXB_CUDA_TRY(ctx, cudaLaunchKernelEx(&cfg, kernel, ma, mb, md, mc, p));
     return DECXB_OK;
 }
 
@@ -982,7 +1022,8 @@ int launch_product(decxb_ctx* ctx, const decxb_fp8_matrix& A, const decxb_fp8_ma
     const int64_t pairs = decxb_ceil_div(p.M, 256) * decxb_ceil_div(p.N, 256), at_once = ctx->sm_count / 2 > 0 ? ctx->sm_count / 2 : 1;
     const double pair_us = 5.0 + (by_row ? 0.80 : 0.42) * (double)decxb_ceil_div(pairs, at_once) * (double)p.num_kb;
     if (cut.us < pair_us) return launch_split<128>(ctx, A, B, p, cut, s);
-    return by_row ? launch<true>(ctx, A, B, p, s) : launch<false>(ctx, A, B, p, s);
+    if (p.C && p.tma_store) return by_row ? launch<true, true>(ctx, A, B, p, s) : launch<false, true>(ctx, A, B, p, s);
+    return by_row ? launch<true, false>(ctx, A, B, p, s) : launch<false, false>(ctx, A, B, p, s);
 }
 
 /* Codes that the copy engine cannot address are copied to a pitch it can. */
@@ -1029,7 +1070,7 @@ int gemm_fp8(decxb_ctx* ctx, const decxb_fp8_matrix* pa, const decxb_fp8_matrix*
         p.sa = view_of(A); p.sb = view_of(B);
         p.C = C; p.ldc = ldc; p.D = D; p.ldd = ldd; p.d_type = d_type;
         /* the copy engine clips a store at the array's edge in whole 16-byte pieces, so N has to be made of them too */
-        p.tma_store = !C && aligned(D, ldd * e, 16) && N * e % 16 == 0;
+        p.tma_store = aligned(D, ldd * e, 16) && (!C || aligned(C, ldc * e, 16)) && N * e % 16 == 0;
         p.d_vec = aligned(D, ldd * e, 4 * e);
         p.wait_limit_ns = ctx->wait_limit_ns; p.status = ctx->d_status;
         rc = launch_product(ctx, A, B, p, s);

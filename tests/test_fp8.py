@@ -139,6 +139,26 @@ def test_product_types_addend_and_results_pitch(ctx, M, N, K, dtype, kinds):
 
 
 @gpu
+@pytest.mark.parametrize("b_rows", [1, 128])
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("M,N,K,pad", [(2055, 1288, 384, 0), (2055, 1288, 300, 1), (2304, 1283, 130, 5), (40, 20000, 260, 8)])
+def test_product_of_many_tiles_with_addend(ctx, M, N, K, pad, dtype, b_rows):
+    """Addend and result through the copy engine (pitch and N of whole 16-byte pieces) and by the threads, in place too."""
+    g = gen(K)
+    A, a = int_matrix(g, M, K, b.FP8_E5M2, 1, pad=-K % 16)
+    B, w = int_matrix(g, N, K, b.FP8_E4M3, b_rows, pad=-K % 16)
+    Cin = torch.randint(-50, 50, (M, N + pad), device=DEV, generator=g).to(dtype)
+    want = (a @ w.t() + Cin[:, :N].double()).to(dtype)
+    assert torch.equal(run_gemm(ctx, A, B, dtype, Cin, pad=8), want)
+    assert torch.equal(run_gemm(ctx, A, B, dtype, None, pad=pad), (a @ w.t()).to(dtype))
+    D = Cin.clone()
+    for _ in range(2):
+        ctx.gemm_fp8(A, B, D, N + pad, Cin=D, ldc=N + pad, stream=cur())
+    ctx.synchronize()
+    assert torch.equal(D[:, :N], (a @ w.t() + want.double()).to(dtype)) and torch.equal(D[:, N:], Cin[:, N:])
+
+
+@gpu
 @pytest.mark.parametrize("M", [3, 200])
 @pytest.mark.parametrize("pad,offset", [(1, 0), (16, 1), (0, 8), (7, 3), (16, 16)])
 def test_product_of_operands_at_any_address_and_pitch(ctx, M, pad, offset):
