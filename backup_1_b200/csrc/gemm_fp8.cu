@@ -296,7 +296,7 @@ __device__ __forceinline__ void put4(const Params& p, int64_t row, int64_t col, 
  * ADDEND : C comes through the copy engine into the boxes that the results leave from, the first of a tile during its
  *          product (4096 x 4096 x 8192 with an fp32 addend: 436 us with the threads' own loads).
  * ------------------------------------------------------------------------------------ */
-template <bool COLVEC>
+template <bool COLVEC, bool ADDEND>
 struct Cfg {
     static constexpr int CTAS = 2;
     static constexpr int BN = 128;                             /* rows of B per CTA */
@@ -308,7 +308,8 @@ struct Cfg {
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
     static constexpr int KB_FLOATS = BM_CTA + (COLVEC ? UMMA_N : 32);
     static constexpr int SCALE_BYTES = SLOTS * KB_FLOATS * 4;
-    static constexpr int BOX_BYTES = EPI_WARPS * 4096;         /* result boxes, one a warp */
+    static constexpr int BOXES = ADDEND ? 2 : 1;               /* result boxes of a warp */
+    static constexpr int BOX_BYTES = EPI_WARPS * BOXES * 4096;
     static constexpr int STAGES = (SMEM_LIMIT - 2048 - SCALE_BYTES - BOX_BYTES) / STAGE_BYTES;
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + BOX_BYTES + SCALE_BYTES + 1024 /* alignment slack */ + 512 /* barriers */;
     static constexpr int BUFS = 512 / UMMA_N;                  /* accumulators in tensor memory */
@@ -323,7 +324,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                       const __grid_constant__ CUtensorMap map_d, const __grid_constant__ CUtensorMap map_c, const Params p)
 {
-    using C = Cfg<COLVEC>;
+    using C = Cfg<COLVEC, ADDEND>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;     /* the swizzle is a function of address bits 4-9 */
     const uint32_t boxes = smem_base + C::STAGES * C::STAGE_BYTES;
@@ -334,8 +335,8 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
     auto tempty_bar = [&](int b) { return bars + 8u * (2 * C::STAGES + b); };
     auto sfull_bar  = [&](int s) { return bars + 8u * (2 * C::STAGES + C::BUFS + s); };
     auto sempty_bar = [&](int s) { return bars + 8u * (2 * C::STAGES + C::BUFS + SLOTS + s); };
-    auto addend_bar = [&](int w) { return bars + 8u * (2 * C::STAGES + C::BUFS + 2 * SLOTS + w); };
-    const uint32_t tmem_slot = bars + 8u * (2 * C::STAGES + C::BUFS + 2 * SLOTS + EPI_WARPS);
+    auto addend_bar = [&](int w) { return bars + 8u * (2 * C::STAGES + C::BUFS + 2 * SLOTS + w); };       /* one a box */
+    const uint32_t tmem_slot = bars + 8u * (2 * C::STAGES + C::BUFS + 2 * SLOTS + 2 * EPI_WARPS);
     auto stage_a = [&](int s) { return smem_base + s * C::STAGE_BYTES; };
     auto stage_b = [&](int s) { return smem_base + s * C::STAGE_BYTES + C::A_BYTES; };
 
@@ -352,7 +353,7 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         for (int s = 0; s < C::STAGES; ++s) { mbar_init(full_bar(s), 1); mbar_init(done_bar(s), 1); }
         for (int b = 0; b < C::BUFS; ++b) mbar_init(tempty_bar(b), EPI_WARPS * C::CTAS);
         for (int s = 0; s < SLOTS; ++s) { mbar_init(sfull_bar(s), 32); mbar_init(sempty_bar(s), EPI_WARPS); }
-        for (int w = 0; w < EPI_WARPS; ++w) mbar_init(addend_bar(w), 1);
+        for (int w = 0; w < 2 * EPI_WARPS; ++w) mbar_init(addend_bar(w), 1);
         fence_barrier_init();
     }
     if (warp == 1) {
@@ -471,14 +472,16 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int q = warp & 3, eh = (warp - 4) >> 2;
         const uint32_t tlane = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(eh * C::ACC);
-        const uint32_t box = boxes + (uint32_t)(warp - 4) * 4096u, cbar = addend_bar(warp - 4);
-        uint32_t cphase = 0;
-        bool pending = false;
-        /* the addend of one box, once the copy engine has read the result that the box held */
-        auto fetch_addend = [&](int64_t col, int64_t row) {
+        const uint32_t box0 = boxes + (uint32_t)(warp - 4) * (4096u * C::BOXES);
+        const int box_cols = p.d_type == DECXB_F32 ? 32 : 64;
+        uint32_t cphase = 0;                          /* parity of each box's addend */
+        uint32_t pending = 0;                         /* boxes with an addend on its way */
+        /* the addend of box i of the tile, once the copy engine has read the results that the box held */
+        auto fetch_addend = [&](int i, int64_t col, int64_t row) {
             tma_store_wait_read<0>();
-            mbar_arrive_expect_tx(cbar, 4096);
-            tma_load_2d(box, &map_c, cbar, (int)col, (int)row);
+            const uint32_t bar = addend_bar((warp - 4) * 2 + (i & 1));
+            mbar_arrive_expect_tx(bar, 4096);
+            tma_load_2d(box0 + (uint32_t)(i & 1) * 4096u, &map_c, bar, (int)col, (int)row);
         };
         int unit = 0, slot = 0, stage = 0;
         uint32_t sphase = 0, phase = 0;
@@ -487,9 +490,13 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
             int tm, tn; tile_coords(t, p.tiles_m, p.tiles_n, p.tile_group, tm, tn);
             const int64_t row0 = (int64_t)tm * C::UMMA_M + cta_rank * BM_CTA + q * 32;
             const int64_t col0 = (int64_t)tn * C::UMMA_N + eh * C::ACC;
-            if (ADDEND && row0 < p.M && col0 < p.N) {
-                if (lane == 0) fetch_addend(col0, row0);
-                pending = true;
+            if (ADDEND && row0 < p.M) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (col0 + i * box_cols < p.N) {
+                        if (lane == 0) fetch_addend(i, col0 + i * box_cols, row0);
+                        pending |= 1u << i;
+                    }
             }
             float sum[C::ACC];
 #pragma unroll
@@ -552,19 +559,19 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
             }
             if (!alive) break;
             if (row0 >= p.M) continue;
-            pending = false;
 #pragma unroll
             for (int c = 0; c < C::ACC; c += 32) {
                 if (col0 + c >= p.N) break;
                 const float* v = sum + c;
                 const bool narrow = p.d_type != DECXB_F32;        /* 64 columns fill a box */
                 if (p.tma_store) {
-                    const int first = narrow && (c & 32) ? 4 : 0;
+                    const int first = narrow && (c & 32) ? 4 : 0, i = narrow ? c >> 6 : c >> 5;
+                    const uint32_t box = box0 + (ADDEND ? (uint32_t)(i & 1) * 4096u : 0u);
                     if (first == 0) {
                         if constexpr (ADDEND) {
-                            if (c > 0 && lane == 0) fetch_addend(col0 + c, row0);       /* the first one came during the product */
-                            if (!warp_wait(cbar, cphase, p, 1700 + warp, t)) { alive = false; break; }
-                            cphase ^= 1u;
+                            if (!warp_wait(addend_bar((warp - 4) * 2 + (i & 1)), (cphase >> (i & 1)) & 1u, p, 1700 + warp, t)) { alive = false; break; }
+                            cphase ^= 1u << (i & 1);
+                            pending &= ~(1u << (i & 1));
                         } else {
                             if (lane == 0) tma_store_wait_read<0>();      /* the box before has been read */
                             __syncwarp();
@@ -578,19 +585,26 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                             tma_store_2d(&map_d, box, (int)(col0 + (narrow ? (c & ~63) : c)), (int)row0);
                             tma_store_commit();
                         }
+                        /* (only fp32 results have more than two boxes) */
+                        if (ADDEND && (i + 2) * box_cols < C::ACC && col0 + (i + 2) * box_cols < p.N) {
+                            if (lane == 0) fetch_addend(i + 2, col0 + (i + 2) * box_cols, row0);
+                            pending |= 1u << (i & 1);
+                        }
                     }
                 } else {
                     __syncwarp();
-                    box_write<COLVEC, false>(DECXB_F32, box, lane, 0, v);
+                    box_write<COLVEC, false>(DECXB_F32, box0, lane, 0, v);
                     __syncwarp();
-                    if (!narrow)                        box_rows<float>(p, box, lane, row0, col0 + c + lane);
-                    else if (p.d_type == DECXB_F16)     box_rows<__half>(p, box, lane, row0, col0 + c + lane);
-                    else                                box_rows<__nv_bfloat16>(p, box, lane, row0, col0 + c + lane);
+                    if (!narrow)                        box_rows<float>(p, box0, lane, row0, col0 + c + lane);
+                    else if (p.d_type == DECXB_F16)     box_rows<__half>(p, box0, lane, row0, col0 + c + lane);
+                    else                                box_rows<__nv_bfloat16>(p, box0, lane, row0, col0 + c + lane);
                 }
             }
         }
-        if (ADDEND && pending && lane == 0)                                 /* a wait gave up: the addend may still be on its way */
-            for (int tries = 0; tries < 2048 && !mbar_try_wait(cbar, cphase); ++tries) __nanosleep(64);
+        if (ADDEND && lane == 0)                                  /* a wait gave up: addends may still be on their way */
+            for (int i = 0; i < 2; ++i)
+                if ((pending >> i) & 1u)
+                    for (int tries = 0; tries < 2048 && !mbar_try_wait(addend_bar((warp - 4) * 2 + i), (cphase >> i) & 1u); ++tries) __nanosleep(64);
         if (p.tma_store && lane == 0) tma_store_wait_all();       /* the box stays until the copy engine is done */
     }
 
@@ -862,7 +876,7 @@ int make_map_fp8(decxb_ctx* ctx, CUtensorMap* map, const decxb_fp8_matrix& m, in
 template <bool COLVEC, bool ADDEND>
 int launch(decxb_ctx* ctx, const decxb_fp8_matrix& A, const decxb_fp8_matrix& B, Params p, cudaStream_t s)
 {
-    using C = Cfg<COLVEC>;
+    using C = Cfg<COLVEC, ADDEND>;
     auto kernel = decxb_gemm_fp8_kernel<COLVEC, ADDEND>;
     static std::once_flag once[DECXB_MAX_DEVICES];
     static cudaError_t attr_err[DECXB_MAX_DEVICES];
