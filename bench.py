@@ -209,7 +209,7 @@ def run_reference(args, wl, name):
             "vs_baseline": None, "dtype": "f32", "data": "synthetic (seeded uniform [-1,1))",
             "config": config_for(args, wl, name, max(args.gpus, 1)), "gpu_launches": 0}
     if not o.ref_cpu_available():
-        print(json.dumps({"impl": "reference", "unavailable": "oracle/_ref/decx_ref_cpu is not built"}))
+        print(json.dumps({"impl": "reference", "unavailable": "oracle/_ref/decx_ref_cpu is not built", "config": base["config"]}))
         return
     try:
         m = cpu_reference_measure(wl, 120.0 / max(args.steps + args.warmup, 1), args.steps + args.warmup)
