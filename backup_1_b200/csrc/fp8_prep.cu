@@ -7,7 +7,6 @@
 #include "tc_ptx.cuh"
 
 #include <mutex>
-#include <new>
 
 namespace {
 
@@ -791,7 +790,7 @@ try {
     DeviceScope dev(ctx);
     if (dev.status) return dev.status;
     return quantize(ctx, x_type, rows, cols, X, ldx, scale_rule, Q, Qt, stream_of(ctx, stream));
-} catch (const std::bad_alloc&) { return DECXB_ERR_ALLOC; }
+} catch (...) { return DECXB_ERR_ALLOC; }      /* the host's memory, or a lock of the runtime */
 
 extern "C" int decxb_rmsnorm(decxb_ctx* ctx, int type, int64_t rows, int64_t cols, const void* X, int64_t ldx,
                              const void* R, int64_t ldr, const void* gamma, int gamma_type, float eps,
@@ -801,7 +800,7 @@ try {
     DeviceScope dev(ctx);
     if (dev.status) return dev.status;
     return norm(ctx, type, rows, cols, X, ldx, R, ldr, gamma, gamma_type, eps, H, ldh, Y, ldy, scale_rule, Q, stream_of(ctx, stream));
-} catch (const std::bad_alloc&) { return DECXB_ERR_ALLOC; }
+} catch (...) { return DECXB_ERR_ALLOC; }      /* the host's memory, or a lock of the runtime */
 
 extern "C" int decxb_rmsnorm_backward_workspace(decxb_ctx* ctx, int64_t rows, int64_t cols, size_t* bytes)
 {
@@ -821,4 +820,4 @@ try {
     if (dev.status) return dev.status;
     return norm_backward(ctx, type, rows, cols, dY, lddy, H, ldh, gamma, gamma_type, eps, dR, lddr, dX, lddx, dgamma, workspace,
                          workspace_bytes, stream_of(ctx, stream));
-} catch (const std::bad_alloc&) { return DECXB_ERR_ALLOC; }
+} catch (...) { return DECXB_ERR_ALLOC; }      /* the host's memory, or a lock of the runtime */

@@ -25,7 +25,6 @@
 #include <cudaTypedefs.h>
 
 #include <mutex>
-#include <new>
 
 namespace {
 
@@ -1058,6 +1057,7 @@ int launch_product(decxb_ctx* ctx, const decxb_fp8_matrix& A, const decxb_fp8_ma
 /* Codes that the copy engine cannot address are copied to a pitch it can. */
 int reachable(decxb_ctx* ctx, decxb_fp8_matrix* m, void** scratch, cudaStream_t s)
 {
+    if (m->rows == 1) m->ld = decxb_ceil_to(m->cols, 16);          /* a single row has no pitch */
     if (aligned(m->data, m->ld, 16)) return DECXB_OK;
     int rc;
     if ((rc = refuse_capture(ctx, s, "an operand's address or ld is not a multiple of 16 bytes"))) return rc;
@@ -1095,7 +1095,7 @@ int gemm_fp8(decxb_ctx* ctx, const decxb_fp8_matrix* pa, const decxb_fp8_matrix*
         Params p = {};
         p.M = M; p.N = N;
         p.num_kb = (int)decxb_ceil_div(A.cols, BK);
-        p.tile_group = 8;
+        p.tile_group = ctx->tile_group > 0 ? ctx->tile_group : 8;
         p.sa = view_of(A); p.sb = view_of(B);
         p.C = C; p.ldc = ldc; p.D = D; p.ldd = ldd; p.d_type = d_type;
         /* the copy engine clips a store at the array's edge in whole 16-byte pieces, so N has to be made of them too */
@@ -1117,4 +1117,4 @@ try {
     DeviceScope dev(ctx);
     if (dev.status) return dev.status;
     return gemm_fp8(ctx, A, B, C, ldc, D, d_type, ldd, stream ? (cudaStream_t)stream : ctx->stream);
-} catch (const std::bad_alloc&) { return DECXB_ERR_ALLOC; }
+} catch (...) { return DECXB_ERR_ALLOC; }      /* the host's memory, or a lock of the runtime */

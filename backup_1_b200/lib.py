@@ -190,7 +190,7 @@ _DTYPES = {"torch.float32": F32, "torch.float16": F16, "torch.bfloat16": BF16,
 _FP8_TYPES = {"torch.float8_e4m3fn": FP8_E4M3, "torch.float8_e5m2": FP8_E5M2}
 
 
-_known_dtypes = {}      # element type objects already looked up by name
+_known_dtypes, _known_fp8 = {}, {}      # element type objects already looked up by name
 
 
 def _dtype(x, given):
@@ -231,20 +231,26 @@ class Fp8Matrix:
     def of(cls, data, scales, block_rows=1):
         """From torch tensors: data [rows][cols] of float8_e4m3fn or float8_e5m2 with contiguous columns, scales
         [ceil(rows / block_rows)][ceil(cols / 128)] of float32 with any strides."""
-        kind = _FP8_TYPES.get(str(data.dtype))
-        if kind is None or str(scales.dtype) != "torch.float32":
-            raise TypeError(f"fp8 matrix of {data.dtype} with scales of {scales.dtype}")
+        kind = _known_fp8.get(data.dtype)
+        if kind is None:
+            kind = _FP8_TYPES.get(str(data.dtype))
+            if kind is None:
+                raise TypeError(f"fp8 matrix of {data.dtype}")
+            _known_fp8[data.dtype] = kind
+        if _dtype(scales, None) != F32:
+            raise TypeError(f"fp8 matrix with scales of {scales.dtype}")
         rows, cols = data.shape
-        if block_rows not in (1, 128) or tuple(scales.shape) != (-(-rows // block_rows), -(-cols // 128)):
+        if block_rows not in (1, 128) or scales.shape != (-(-rows // block_rows), -(-cols // 128)):
             raise ValueError(f"scales of shape {tuple(scales.shape)} for {rows} x {cols} codes in blocks of {block_rows} x 128")
-        if cols > 1 and data.stride(1) != 1:
+        ld, step = data.stride()
+        if cols > 1 and step != 1:
             raise ValueError("the codes of a row must be contiguous")
-        if rows > 1 and data.stride(0) < cols:
+        if rows <= 1:
+            ld = -(-cols // 16) * 16        # a single row has no pitch
+        elif ld < cols:
             raise ValueError("rows of codes overlap")
-        ld = data.stride(0) if rows > 1 else cols
-        if rows == 1 and ld % 16:
-            ld = -(-ld // 16) * 16          # a single row has no pitch: give it one that the copy engine can take
-        return cls(data, scales, rows, cols, ld, scales.stride(0), scales.stride(1), block_rows, kind)
+        srs, sbs = scales.stride()
+        return cls(data, scales, rows, cols, ld, srs, sbs, block_rows, kind)
 
     @classmethod
     def empty(cls, rows, cols, block_rows=1, type=FP8_E4M3, device="cuda:0"):

@@ -713,6 +713,127 @@ def test_capture_refuses_what_needs_scratch(ctx):
 
 
 @gpu
+def test_pitches_and_offsets_beyond_32_bits(ctx):
+    """Three rows 2^31 + 64 elements apart, and results that far apart, in every operator."""
+    far, rows, cols = 2 ** 31 + 64, 3, 640
+    g = gen(4)
+    x = torch.randn(rows, cols, device=DEV, generator=g).to(torch.bfloat16)
+    gamma = torch.ones(cols, device=DEV)
+    apart = torch.empty(2 * far + cols, device=DEV, dtype=torch.bfloat16)
+
+    def view(t):
+        return torch.as_strided(t, (rows, cols), (far, 1))
+    view(apart).copy_(x)
+    out = torch.empty_like(apart)
+    Y, Q, T = torch.empty_like(x), b.Fp8Matrix.empty(rows, cols), b.Fp8Matrix.empty(cols, rows)
+    ctx.rmsnorm(rows, cols, x, cols, gamma, 1e-6, Y=Y, ldy=cols, Q=Q, stream=cur())
+    ctx.rmsnorm(rows, cols, apart, far, gamma, 1e-6, Y=out, ldy=far, stream=cur())
+    assert torch.equal(view(out), Y)
+    dx = torch.empty_like(x)
+    ctx.rmsnorm_backward(rows, cols, Y, cols, x, cols, gamma, 1e-6, dx, cols, stream=cur())
+    ctx.rmsnorm_backward(rows, cols, out, far, apart, far, gamma, 1e-6, out, far, stream=cur())
+    assert torch.equal(view(out), dx)
+    codes = torch.empty(2 * far + cols, device=DEV, dtype=torch.float8_e4m3fn)
+    F = b.Fp8Matrix(codes, torch.empty(rows * 5, device=DEV), rows, cols, far, 5, 1)
+    ctx.quantize_fp8(rows, cols, apart, far, F, T, stream=cur())
+    ctx.quantize_fp8(rows, cols, x, cols, Q, stream=cur())
+    ctx.synchronize()
+    assert torch.equal(view(codes).view(torch.uint8), Q.data.view(torch.uint8)) and torch.equal(F.scales.view(rows, 5), Q.scales)
+    W, w = int_matrix(g, 256, cols, b.FP8_E4M3, 128)
+    near, dist = torch.empty(rows, 256, device=DEV, dtype=torch.bfloat16), apart
+    ctx.gemm_fp8(Q, W, near, 256, stream=cur())
+    ctx.gemm_fp8(F, W, dist, far, stream=cur())
+    ctx.gemm_fp8(F, W, dist, far, Cin=dist, ldc=far, stream=cur())
+    ctx.synchronize()
+    assert torch.equal(torch.as_strided(dist, (rows, 256), (far, 1)), (near.float() * 2).bfloat16())
+
+
+_FIRST_CALL_CAPTURED = r"""
+import torch
+import backup_1_b200 as b
+ctx = b.Context(0)
+t, w, o = 130, 512, 384
+x, g = torch.randn(t, w, device="cuda").bfloat16(), torch.ones(w, device="cuda")
+W = torch.randn(o, w, device="cuda")
+q, wq, out = b.Fp8Matrix.empty(t, w), b.Fp8Matrix.empty(o, w, 128), torch.zeros(t, o, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    s = torch.cuda.current_stream()
+    ctx.quantize_fp8(o, w, W, w, wq, stream=s)
+    ctx.rmsnorm(t, w, x, w, g, 1e-6, Q=q, stream=s)
+    ctx.gemm_fp8(q, wq, out, o, stream=s)
+graph.replay()
+torch.cuda.synchronize()
+ctx.synchronize()
+first = out.clone()
+assert float(first.abs().max()) > 0
+ctx.quantize_fp8(o, w, W, w, wq, stream=torch.cuda.current_stream())
+ctx.rmsnorm(t, w, x, w, g, 1e-6, Q=q, stream=torch.cuda.current_stream())
+ctx.gemm_fp8(q, wq, out, o, stream=torch.cuda.current_stream())
+torch.cuda.synchronize()
+assert torch.equal(first, out)
+print("captured first call ok")
+"""
+
+
+@gpu
+def test_the_first_call_of_a_process_may_be_captured():
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    r = subprocess.run([sys.executable, "-c", _FIRST_CALL_CAPTURED], cwd=Path(__file__).resolve().parents[1], capture_output=True,
+                       text=True, timeout=300)
+    assert r.returncode == 0 and "captured first call ok" in r.stdout, r.stdout[-1000:] + r.stderr[-2000:]
+
+
+@gpu
+def test_two_threads_call_at_once(ctx):
+    """Two host threads, each with its own stream, on one context: the results of either alone."""
+    import threading
+
+    layers = [Layer(ctx, 300, 384, 512, seed) for seed in (5, 6)]
+    want = []
+    for v in layers:
+        v.step()
+        torch.cuda.synchronize()
+        want.append(v.results())
+    streams = [torch.cuda.Stream() for _ in layers]
+    failures = []
+
+    def work(v, s):
+        try:
+            with torch.cuda.stream(s):
+                for _ in range(20):
+                    v.dw.fill_(1.0)
+                    v.step()
+        except Exception as e:       # noqa: BLE001
+            failures.append(e)
+    threads = [threading.Thread(target=work, args=a) for a in zip(layers, streams)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    ctx.synchronize()
+    assert not failures, failures
+    for v, w in zip(layers, want):
+        for a, c in zip(v.results(), w):
+            assert torch.equal(a, c)
+
+
+@gpu
+def test_the_callers_device_is_left_and_errors_have_a_text(ctx):
+    L = ctx.L
+    before = torch.cuda.current_device()
+    A = b.Fp8Matrix.empty(4, 256)
+    assert L.decxb_gemm_fp8(ctx.h, A.addr, A.addr, None, 0, None, 0, 4, None) == 13
+    assert b"D: null" in L.decxb_last_error(ctx.h)
+    assert torch.cuda.current_device() == before
+
+
+@gpu
 def test_calls_on_the_contexts_own_stream_and_on_another(ctx):
     """Without a stream the context's own is used, after torch's current one; with one, the work is ordered on it."""
     layer = Layer(ctx, 64, 256, 128)
