@@ -40,6 +40,31 @@ int launch_after(decxb_ctx* ctx, void (*kernel)(P...), unsigned grid, dim3 threa
     return DECXB_OK;
 }
 
+/* Bulk copy of `bytes` (a multiple of 16, both addresses too) to shared memory, counted on an mbarrier. */
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 :: "r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+/* Wait for a stage's copies; where they do not come within the limit, the status word says so and the wait ends. */
+__device__ __forceinline__ void wait_copy(uint32_t bar, uint32_t parity, long long limit_ns, decxb_dev_status* status)
+{
+    unsigned long long t0 = 0;
+    for (uint32_t spins = 1; !tcptx::mbar_try_wait(bar, parity); ++spins) {
+        if (spins & 1023u) continue;
+        const unsigned long long t = tcptx::globaltimer_ns();
+        if (t0 == 0) t0 = t;
+        if ((long long)(t - t0) > limit_ns) {
+            if (atomicCAS(&status->code, 0, DECXB_DEVERR_WAIT_EXPIRED) == 0) {
+                status->where = 3000; status->block = (int)blockIdx.x; status->detail = 0;
+                __threadfence_system();
+            }
+            return;
+        }
+    }
+}
+
 /* ---- root-mean-square norm ---------------------------------------------------------------
  * One block per row, or eight rows of up to 256 columns with a warp each.  A thread holds VPT vectors of eight consecutive
  * columns, vector i * blockDim + tid, so the 16 lanes of half a warp cover one 128-column block of the row and its
@@ -133,6 +158,67 @@ decxb_rmsnorm_kernel(const NormArgs a)
     }
 }
 
+/* Many rows of up to 4096 columns: a block walks rows blockIdx, blockIdx + gridDim, ... that bulk copies bring to shared memory
+ * `stages` rows ahead, one vector a thread.  Against a block per row (above) there is always something on the way, and
+ * what does not depend on the row (gamma, addresses) is done once: the instructions of 16-bit rows bound that
+ * kernel (43 an element, 73 % of the issue slots). */
+template <typename T>
+__global__ void __launch_bounds__(512, 2)
+decxb_rmsnorm_rows_kernel(const NormArgs a, const int stages, const long long wait_limit_ns, decxb_dev_status* status)
+{
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float part[2][16];
+    __shared__ __align__(8) uint64_t bars[8];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nwarps = blockDim.x >> 5, cols = (int)a.cols;
+    const int arrays = a.r ? 2 : 1;
+    const uint32_t row_bytes = (uint32_t)cols * (uint32_t)sizeof(T);
+    const int first = tid * 8, n = first < cols ? 8 : 0;
+    auto fetch = [&](int64_t row, int st) {
+        const uint32_t bar = tcptx::smem_u32(&bars[st]), at = tcptx::smem_u32(smem) + (uint32_t)(st * arrays) * row_bytes;
+        tcptx::mbar_arrive_expect_tx(bar, row_bytes * arrays);
+        bulk_load(at, static_cast<const T*>(a.x) + row * a.ldx, row_bytes, bar);
+        if (a.r) bulk_load(at + row_bytes, static_cast<const T*>(a.r) + row * a.ldr, row_bytes, bar);
+    };
+    if (tid == 0) {
+        for (int st = 0; st < stages; ++st) tcptx::mbar_init(tcptx::smem_u32(&bars[st]), 1);
+        tcptx::fence_barrier_init();
+    }
+    __syncthreads();
+    start_after_previous();
+    if (tid == 0)
+        for (int st = 0; st < stages; ++st)
+            if (blockIdx.x + (int64_t)st * gridDim.x < a.rows) fetch(blockIdx.x + (int64_t)st * gridDim.x, st);
+    float g[8];
+    load8_any(a.gamma, a.gamma_type, first, n, true, g);
+    const float of_cols = 1.0f / (float)cols;
+    int st = 0, turn = 0; uint32_t phase = 0;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+        wait_copy(tcptx::smem_u32(&bars[st]), phase, wait_limit_ns, status);
+        const T* in = reinterpret_cast<const T*>(smem + (size_t)(st * arrays) * row_bytes);
+        float v[8], sum = 0.0f;
+        load8(in + first, n, true, v);
+        if (a.r) {
+            float w[8];
+            load8(in + cols + first, n, true, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] += w[j];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum = fmaf(v[j], v[j], sum);
+        sum = warp_sum(sum);
+        if (lane == 0) part[turn][warp] = sum;
+        __syncthreads();                       /* every thread has its values: the stage can be filled again */
+        if (tid == 0 && row + (int64_t)stages * gridDim.x < a.rows) fetch(row + (int64_t)stages * gridDim.x, st);
+        const float rstd = rsqrtf(warp_sum(lane < nwarps ? part[turn][lane] : 0.0f) * of_cols + a.eps);
+        if (a.h && n) store8(static_cast<T*>(a.h) + row * a.ldh + first, 8, true, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = v[j] * rstd * g[j];
+        if (a.y && n) store8(static_cast<T*>(a.y) + row * a.ldy + first, 8, true, v);
+        if (a.q) quantise_row8(a, a.q + row * a.ldq, a.s + row * a.srs, first, n, v);
+        if (++st == stages) { st = 0; phase ^= 1u; }
+    }
+}
+
 /* Rows too long for the registers: the row is read twice (the second time from L2, mostly). */
 template <typename T>
 __global__ void __launch_bounds__(1024)
@@ -197,12 +283,31 @@ int launch_norm_rows(decxb_ctx* ctx, const NormArgs& a, int64_t nvec, cudaStream
                  : launch_after(ctx, decxb_rmsnorm_kernel<T, VPT, false>, grid, dim3(threads, rows), 0, s, a);
 }
 
+template <typename T>
+int launch_norm_many(decxb_ctx* ctx, const NormArgs& a, cudaStream_t s)
+{
+    auto kernel = decxb_rmsnorm_rows_kernel<T>;
+    const int stages = 4;
+    const size_t smem = (size_t)stages * a.cols * sizeof(T) * (a.r ? 2 : 1);      /* at most 64 KiB */
+    static std::once_flag once[DECXB_MAX_DEVICES];
+    static cudaError_t err[DECXB_MAX_DEVICES];
+    std::call_once(once[ctx->device], [&] { err[ctx->device] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024); });
+    if (err[ctx->device] != cudaSuccess) return decxb_fail(ctx, DECXB_ERR_CUDA, std::string("norm kernel attributes: ") + cudaGetErrorString(err[ctx->device]));
+    return launch_after(ctx, kernel, (unsigned)(2 * ctx->sm_count), threads_for(decxb_ceil_div(a.cols, 8), 1, 512), smem, s, a, stages,
+                        ctx->wait_limit_ns, ctx->d_status);
+}
+
 /* One vector a thread as far as 1024 threads reach (8192 x 4096 bf16 with one, two, four: 64, 69, 74 us): a block's loads,
  * sum and stores follow one another, so it is the number of blocks on an SM that keeps the memory busy. */
 template <typename T>
 int launch_norm(decxb_ctx* ctx, const NormArgs& a, cudaStream_t s)
 {
     const int64_t nvec = decxb_ceil_div(a.cols, 8);
+    /* 16-bit rows of 2049 to 4096 columns, eight or more to an SM: 8192 x 4096 60.6 us with a block a row, 51.8 with rows by bulk
+     * copies; but 600 x 4096 5.6 and 7.0, 16384 x 1024 29 and 58, 4096 x 4096 fp32 46.6 and 53.8 */
+    if constexpr (sizeof(T) == 2)
+        if (a.vec && a.gvec && a.cols % 8 == 0 && (!a.q || a.qvec) && a.cols > 2048 && a.cols <= 4096 && a.rows >= 8 * (int64_t)ctx->sm_count)
+            return launch_norm_many<T>(ctx, a, s);
     if (nvec <= 1024) return launch_norm_rows<T, 1>(ctx, a, nvec, s);
     if (nvec <= 2048) return launch_norm_rows<T, 2>(ctx, a, nvec, s);
     if (nvec <= 4096) return launch_norm_rows<T, 4>(ctx, a, nvec, s);
@@ -240,31 +345,6 @@ __device__ __forceinline__ void backward8(const float* w, const float* x, const 
     for (int j = 0; j < 8; ++j) {
         acc[j] = fmaf(w[j], x[j] * r, acc[j]);
         o[j] = fmaf(r, w[j] * g[j] - x[j] * k, o[j]);
-    }
-}
-
-/* Bulk copy of `bytes` (a multiple of 16, both addresses too) to shared memory, counted on an mbarrier. */
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar)
-{
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 :: "r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
-}
-
-/* Wait for a stage's copies; where they do not come within the limit, the status word says so and the wait ends. */
-__device__ __forceinline__ void wait_copy(uint32_t bar, uint32_t parity, long long limit_ns, decxb_dev_status* status)
-{
-    unsigned long long t0 = 0;
-    for (uint32_t spins = 1; !tcptx::mbar_try_wait(bar, parity); ++spins) {
-        if (spins & 1023u) continue;
-        const unsigned long long t = tcptx::globaltimer_ns();
-        if (t0 == 0) t0 = t;
-        if ((long long)(t - t0) > limit_ns) {
-            if (atomicCAS(&status->code, 0, DECXB_DEVERR_WAIT_EXPIRED) == 0) {
-                status->where = 3000; status->block = (int)blockIdx.x; status->detail = 0;
-                __threadfence_system();
-            }
-            return;
-        }
     }
 }
 
@@ -611,11 +691,11 @@ decxb_quantize_fp8_kernel(const QuantArgs a)
             if ((t & 1) == 0 && (t >> 1) < nr) a.q.s[(row + (t >> 1)) * a.q.srs + tile_c * a.q.sbs] = s;
         }
         Quantiser z = quantiser(s);
-        const float s_row = z.s, inv_row = z.inv;
+        const float s_row = z.minus_s, inv_row = z.inv;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             if (a.q.block_rows == 1) {
-                z.s = __shfl_sync(0xffffffffu, s_row, 2 * i, 16);
+                z.minus_s = __shfl_sync(0xffffffffu, s_row, 2 * i, 16);
                 z.inv = __shfl_sync(0xffffffffu, inv_row, 2 * i, 16);
             }
             float v[8];

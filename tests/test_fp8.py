@@ -381,7 +381,8 @@ def test_quantise_refusals(ctx):
 
 
 # ---- norm ---------------------------------------------------------------------------------------------------------------
-NORM_SHAPES = [(1, 1), (1, 8), (3, 7), (5, 128), (2, 130), (9, 1000), (1, 4096), (4, 4100), (3, 8192), (2, 16384), (2, 33000), (1, 40001), (1200, 64)]
+NORM_SHAPES = [(1, 1), (1, 8), (3, 7), (5, 128), (2, 130), (9, 1000), (1, 4096), (4, 4100), (3, 8192), (2, 16384), (2, 33000), (1, 40001), (1200, 64),
+               (1300, 2056), (1190, 4096)]
 # roundings of one value: at most 64 terms in a thread's chain of squares (fewer outside the longest rows), 10 levels of
 # shuffles, mean, eps, the reciprocal root's 2 steps, three products: under 96
 NORM_U = 96 * U
@@ -454,6 +455,27 @@ def test_norm_strides_in_place_and_single_outputs(ctx, cols, pad, offset):
     ctx.rmsnorm(rows, cols, x, cols, gamma, 0.0, R=vr2, ldr=ld, Q=q2, stream=cur())                          # codes alone
     ctx.synchronize()
     assert torch.equal(vx[:, :cols], Y) and torch.equal(q2.data.view(torch.uint8), Q.data.view(torch.uint8)) and torch.equal(q2.scales, Q.scales)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_norm_of_many_rows_in_place(ctx, dtype):
+    """As many rows as are walked by blocks that fetch ahead: nothing is read after it was overwritten."""
+    rows, cols = 3001, 2304
+    g = gen(9)
+    x, r = (torch.randn(rows, cols, device=DEV, generator=g).to(dtype) for _ in range(2))
+    gamma = torch.randn(cols, device=DEV, generator=g)
+    H, Y = torch.empty_like(x), torch.empty_like(x)
+    ctx.rmsnorm(rows, cols, x, cols, gamma, 1e-5, R=r, ldr=cols, H=H, ldh=cols, Y=Y, ldy=cols, stream=cur())
+    h, y = norm_ref(x, r, gamma, 1e-5)
+    assert near(H, h, dtype, 2 * U) and near(Y, y, dtype, NORM_U)
+    x2, r2 = x.clone(), r.clone()
+    ctx.rmsnorm(rows, cols, x2, cols, gamma, 1e-5, R=r2, ldr=cols, H=r2, ldh=cols, Y=x2, ldy=cols, stream=cur())
+    ctx.synchronize()
+    assert torch.equal(r2, H) and torch.equal(x2, Y)
+    one = torch.empty_like(x)
+    ctx.rmsnorm(rows, cols, x, cols, gamma, 1e-5, Y=one, ldy=cols, stream=cur())                # without a residual
+    assert near(one, norm_ref(x, None, gamma, 1e-5)[1], dtype, NORM_U)
 
 
 @gpu
