@@ -225,7 +225,10 @@ class Fp8Matrix:
         self.c = Fp8MatrixStruct(_ptr(data), _ptr(scales), rows, cols, ld, scale_row_stride, scale_block_stride, type, block_rows)
         self.addr = C.addressof(self.c)
         self.rows, self.cols, self.block_rows, self.type = rows, cols, block_rows, type
-        self.devices = tuple(t.get_device() for t in (data, scales) if hasattr(t, "get_device"))
+        on = {t.get_device() for t in (data, scales) if hasattr(t, "get_device")}
+        if len(on) > 1:
+            raise ValueError("codes and scales on different devices")
+        self.device = on.pop() if on else None         # of the tensors; None: raw addresses
 
     @classmethod
     def of(cls, data, scales, block_rows=1):
@@ -393,58 +396,62 @@ class Context:
         self._chk(self.L.decxb_gemm_release_b(self.h, pb, stream))
 
     # -- 8-bit linear layer -----------------------------------------------------------------
-    def _at(self, x):
-        """Address of an array argument; a tensor has to lie on the context's device (a raw address is the caller's word)."""
+    def _array(self, x, element):
+        """Address of an array argument of F32 / F16 / BF16 elements (None: of any type).  A tensor has to hold those and lie on
+        the context's device; a raw address is the caller's word."""
         if x is None:
             return None
         try:
-            on = x.get_device()
-        except AttributeError:
-            return _ptr(x)
-        if on != self.device:
+            if x.get_device() == self.device and (element is None or _known_dtypes[x.dtype] == element):
+                return x.data_ptr()
+        except (AttributeError, KeyError):
+            pass
+        if element is not None:
+            _dtype(x, element)
+        if hasattr(x, "get_device") and x.get_device() != self.device:
             raise DecxbError(13, f"a tensor on {x.device} was passed to a context of cuda:{self.device}")
-        return x.data_ptr()
+        return _ptr(x)
 
     def _fp8(self, m):
         """Address of an fp8 matrix argument's descriptor."""
         if m is None:
             return None
-        for on in m.devices:
-            if on != self.device:
-                raise DecxbError(13, f"an fp8 matrix on device {on} was passed to a context of cuda:{self.device}")
+        if m.device != self.device and m.device is not None:
+            raise DecxbError(13, f"an fp8 matrix on device {m.device} was passed to a context of cuda:{self.device}")
         return m.addr
 
     def _on(self, stream, some_tensor):
         """Handle of a `stream` argument.  Without one the work runs on the context's own stream, after what torch has queued."""
-        if stream is None and getattr(some_tensor, "is_cuda", False):
-            import torch
+        if stream is None:
+            if getattr(some_tensor, "is_cuda", False):
+                import torch
 
-            torch.cuda.current_stream(some_tensor.device).synchronize()
+                torch.cuda.current_stream(some_tensor.device).synchronize()
+            return None
         return _stream(stream)
 
     def gemm_fp8(self, A: Fp8Matrix, B: Fp8Matrix, D, ldd, Cin=None, ldc=0, d_type=None, stream=None):
         """D[A.rows][B.rows] = A B^T (+ Cin), both operands K-contiguous with their block scales (decxb_gemm_fp8)."""
-        t = _dtype(D, d_type)
-        if Cin is not None:
-            _dtype(Cin, t)
-        self._chk(self.L.decxb_gemm_fp8(self.h, self._fp8(A), self._fp8(B), self._at(Cin), ldc, self._at(D), t, ldd,
-                                        self._on(stream, A.data)))
+        t, at = _dtype(D, d_type), self._array
+        rc = self.L.decxb_gemm_fp8(self.h, self._fp8(A), self._fp8(B), at(Cin, t), ldc, at(D, t), t, ldd, self._on(stream, A.data))
+        if rc:
+            self._chk(rc)
 
     def quantize_fp8(self, rows, cols, X, ldx, Q: Fp8Matrix = None, Qt: Fp8Matrix = None, rule=SCALE_AMAX, x_type=None, stream=None):
         """X [rows][cols] into Q and / or, transposed, into Qt (decxb_quantize_fp8)."""
-        self._chk(self.L.decxb_quantize_fp8(self.h, _dtype(X, x_type), rows, cols, self._at(X), ldx, rule, self._fp8(Q), self._fp8(Qt),
-                                            self._on(stream, X)))
+        t = _dtype(X, x_type)
+        rc = self.L.decxb_quantize_fp8(self.h, t, rows, cols, self._array(X, t), ldx, rule, self._fp8(Q), self._fp8(Qt), self._on(stream, X))
+        if rc:
+            self._chk(rc)
 
     def rmsnorm(self, rows, cols, X, ldx, gamma, eps, R=None, ldr=0, H=None, ldh=0, Y=None, ldy=0, Q: Fp8Matrix = None,
                 rule=SCALE_AMAX, type=None, gamma_type=None, stream=None):
         """h = X (+ R), y = h / rms(h) * gamma into H, Y and, quantised, Q, whichever are given (decxb_rmsnorm)."""
-        t = _dtype(X, type)
-        for a in (R, H, Y):
-            if a is not None:
-                _dtype(a, t)
-        self._chk(self.L.decxb_rmsnorm(self.h, t, rows, cols, self._at(X), ldx, self._at(R), ldr, self._at(gamma),
-                                       _dtype(gamma, gamma_type), eps, self._at(H), ldh, self._at(Y), ldy, rule, self._fp8(Q),
-                                       self._on(stream, X)))
+        t, tg, at = _dtype(X, type), _dtype(gamma, gamma_type), self._array
+        rc = self.L.decxb_rmsnorm(self.h, t, rows, cols, at(X, t), ldx, at(R, t), ldr, at(gamma, tg), tg, eps, at(H, t), ldh, at(Y, t), ldy,
+                                  rule, self._fp8(Q), self._on(stream, X))
+        if rc:
+            self._chk(rc)
 
     def rmsnorm_backward_workspace(self, rows, cols) -> int:
         n = _sz()
@@ -454,15 +461,11 @@ class Context:
     def rmsnorm_backward(self, rows, cols, dY, lddy, H, ldh, gamma, eps, dX, lddx, dgamma=None, dR=None, lddr=0,
                          workspace=None, workspace_bytes=0, type=None, gamma_type=None, stream=None):
         """Gradients of rmsnorm's y: dX (with dR added) and dgamma, fp32 (decxb_rmsnorm_backward)."""
-        t = _dtype(H, type)
-        for a in (dY, dX, dR):
-            if a is not None:
-                _dtype(a, t)
-        if dgamma is not None:
-            _dtype(dgamma, F32)
-        self._chk(self.L.decxb_rmsnorm_backward(self.h, t, rows, cols, self._at(dY), lddy, self._at(H), ldh, self._at(gamma),
-                                                _dtype(gamma, gamma_type), eps, self._at(dR), lddr, self._at(dX), lddx, self._at(dgamma),
-                                                self._at(workspace), workspace_bytes, self._on(stream, gamma)))
+        t, tg, at = _dtype(H, type), _dtype(gamma, gamma_type), self._array
+        rc = self.L.decxb_rmsnorm_backward(self.h, t, rows, cols, at(dY, t), lddy, at(H, t), ldh, at(gamma, tg), tg, eps, at(dR, t), lddr,
+                                           at(dX, t), lddx, at(dgamma, F32), at(workspace, None), workspace_bytes, self._on(stream, gamma))
+        if rc:
+            self._chk(rc)
 
     # -- convolution ----------------------------------------------------------------------
     def set_pack_variant(self, variant: int):

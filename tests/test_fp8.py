@@ -247,6 +247,10 @@ def test_product_refusals(ctx):
     assert ctx.L.decxb_gemm_fp8(ctx.h, None, B.addr, None, 0, D.data_ptr(), 0, 8, None) == 13
     with pytest.raises(TypeError):
         ctx.gemm_fp8(A, B, D, 8, Cin=D.half(), ldc=8)
+    with pytest.raises(b.DecxbError):
+        ctx.gemm_fp8(b.Fp8Matrix.empty(4, 256, device="cpu"), B, D, 8)
+    with pytest.raises(ValueError):
+        b.Fp8Matrix.of(A.data, A.scales.cpu())
     assert bool((D == 0).all())
 
 
