@@ -303,7 +303,7 @@ __device__ __forceinline__ void put4(const Params& p, int64_t row, int64_t col, 
  * ADDEND : C comes through the copy engine into the boxes that the results leave from, the first of a tile during its
  *          product (4096 x 4096 x 8192 with an fp32 addend: 222 us, with the threads' own loads 436).
  * ------------------------------------------------------------------------------------ */
-template <bool COLVEC, bool ADDEND>
+template <bool COLVEC>
 struct Cfg {
     static constexpr int CTAS = 2;
     static constexpr int BN = 128;                             /* rows of B per CTA */
@@ -315,7 +315,7 @@ struct Cfg {
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
     static constexpr int KB_FLOATS = BM_CTA + (COLVEC ? UMMA_N : 32);
     static constexpr int SCALE_BYTES = SLOTS * KB_FLOATS * 4;
-    static constexpr int BOXES = ADDEND ? 2 : 1;               /* result boxes of a warp */
+    static constexpr int BOXES = 2;                            /* result boxes of a warp, one filled while the other is read */
     static constexpr int BOX_BYTES = EPI_WARPS * BOXES * 4096;
     static constexpr int STAGES = (SMEM_LIMIT - 2048 - SCALE_BYTES - BOX_BYTES) / STAGE_BYTES;
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + BOX_BYTES + SCALE_BYTES + 1024 /* alignment slack */ + 512 /* barriers */;
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                       const __grid_constant__ CUtensorMap map_d, const __grid_constant__ CUtensorMap map_c, const Params p)
 {
-    using C = Cfg<COLVEC, ADDEND>;
+    using C = Cfg<COLVEC>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;     /* the swizzle is a function of address bits 4-9 */
     const uint32_t boxes = smem_base + C::STAGES * C::STAGE_BYTES;
@@ -482,6 +482,7 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
         const uint32_t box0 = boxes + (uint32_t)(warp - 4) * (4096u * C::BOXES);
         const int box_cols = p.d_type == DECXB_F32 ? 32 : 64;
         uint32_t cphase = 0;                          /* parity of each box's addend */
+        uint32_t turn = 0;                            /* boxes stored so far */
         uint32_t pending = 0;                         /* boxes with an addend on its way */
         /* the addend of box i of the tile, once the copy engine has read the results that the box held */
         auto fetch_addend = [&](int i, int64_t col, int64_t row) {
@@ -574,14 +575,14 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                 const bool narrow = p.d_type != DECXB_F32;        /* 64 columns fill a box */
                 if (p.tma_store) {
                     const int first = narrow && (c & 32) ? 4 : 0, i = narrow ? c >> 6 : c >> 5;
-                    const uint32_t box = box0 + (ADDEND ? (uint32_t)(i & 1) * 4096u : 0u);
+                    const uint32_t box = box0 + (uint32_t)((ADDEND ? i : (int)turn) & 1) * 4096u;
                     if (first == 0) {
                         if constexpr (ADDEND) {
                             if (!warp_wait(addend_bar((warp - 4) * 2 + (i & 1)), (cphase >> (i & 1)) & 1u, p, 1700 + warp, t)) { alive = false; break; }
                             cphase ^= 1u << (i & 1);
                             pending &= ~(1u << (i & 1));
                         } else {
-                            if (lane == 0) tma_store_wait_read<0>();      /* the box before has been read */
+                            if (lane == 0) tma_store_wait_read<1>();      /* what this box held has been read */
                             __syncwarp();
                         }
                     }
@@ -593,6 +594,7 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                             tma_store_2d(&map_d, box, (int)(col0 + (narrow ? (c & ~63) : c)), (int)row0);
                             tma_store_commit();
                         }
+                        ++turn;
                         /* (only fp32 results have more than two boxes) */
                         if (ADDEND && (i + 2) * box_cols < C::ACC && col0 + (i + 2) * box_cols < p.N) {
                             if (lane == 0) fetch_addend(i + 2, col0 + (i + 2) * box_cols, row0);
@@ -886,7 +888,7 @@ int make_map_fp8(decxb_ctx* ctx, CUtensorMap* map, const decxb_fp8_matrix& m, in
 template <bool COLVEC, bool ADDEND>
 int launch(decxb_ctx* ctx, const decxb_fp8_matrix& A, const decxb_fp8_matrix& B, Params p, cudaStream_t s)
 {
-    using C = Cfg<COLVEC, ADDEND>;
+    using C = Cfg<COLVEC>;
     auto kernel = decxb_gemm_fp8_kernel<COLVEC, ADDEND>;
     static std::once_flag once[DECXB_MAX_DEVICES];
     static cudaError_t attr_err[DECXB_MAX_DEVICES];
