@@ -19,6 +19,23 @@ template <> __device__ __forceinline__ float from_f32<float>(float x) { return x
 template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+/* The two elements of a 32-bit word as floats (bf16: one instruction each, where a conversion of the halves takes two). */
+__device__ __forceinline__ void halves(uint32_t w, const __nv_bfloat16*, float& a, float& b)
+{
+    a = __uint_as_float(w << 16); b = __uint_as_float(w & 0xffff0000u);
+}
+__device__ __forceinline__ void halves(uint32_t w, const __half*, float& a, float& b)
+{
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    a = f.x; b = f.y;
+}
+template <typename T>
+__device__ __forceinline__ void unpack4(const uint4& u, float* v)
+{
+    const T* const kind = nullptr;
+    halves(u.x, kind, v[0], v[1]); halves(u.y, kind, v[2], v[3]); halves(u.z, kind, v[4], v[5]); halves(u.w, kind, v[6], v[7]);
+}
+
 /* Eight consecutive elements of a row as floats.  `n` of them exist (the others read as 0); `vec`: the
  * address is 16-byte aligned, so a whole vector moves in 128-bit accesses. */
 template <typename T>
@@ -29,10 +46,7 @@ __device__ __forceinline__ void load8(const T* p, int n, bool vec, float* v)
             const float4 a = *reinterpret_cast<const float4*>(p), b = *(reinterpret_cast<const float4*>(p) + 1);
             v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
         } else {
-            const uint4 u = *reinterpret_cast<const uint4*>(p);
-            const T* e = reinterpret_cast<const T*>(&u);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = to_f32(e[j]);
+            unpack4<T>(*reinterpret_cast<const uint4*>(p), v);
         }
     } else {
 #pragma unroll
@@ -57,9 +71,23 @@ __device__ __forceinline__ void load_raw(const T* p, int n, bool vec, Raw8<T>& o
 template <typename T>
 __device__ __forceinline__ void unpack(const Raw8<T>& r, float* v)
 {
-    const T* e = reinterpret_cast<const T*>(r.u);
+    if constexpr (sizeof(T) == 2) unpack4<T>(r.u[0], v);
+    else {
+        const float* e = reinterpret_cast<const float*>(r.u);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = to_f32(e[j]);
+        for (int j = 0; j < 8; ++j) v[j] = e[j];
+    }
+}
+
+__device__ __forceinline__ uint32_t joined(float a, float b, const __nv_bfloat16*)
+{
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t joined(float a, float b, const __half*)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 template <typename T>
@@ -70,11 +98,8 @@ __device__ __forceinline__ void store8(T* p, int n, bool vec, const float* v)
             *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
             *(reinterpret_cast<float4*>(p) + 1) = make_float4(v[4], v[5], v[6], v[7]);
         } else {
-            uint4 u;
-            T* e = reinterpret_cast<T*>(&u);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) e[j] = from_f32<T>(v[j]);
-            *reinterpret_cast<uint4*>(p) = u;
+            const T* const kind = nullptr;
+            *reinterpret_cast<uint4*>(p) = make_uint4(joined(v[0], v[1], kind), joined(v[2], v[3], kind), joined(v[4], v[5], kind), joined(v[6], v[7], kind));
         }
     } else {
 #pragma unroll

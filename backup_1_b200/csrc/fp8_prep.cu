@@ -161,9 +161,12 @@ decxb_rmsnorm_kernel(const NormArgs a)
 /* Many rows of up to 4096 columns: a block walks rows blockIdx, blockIdx + gridDim, ... that bulk copies bring to shared memory
  * `stages` rows ahead, one vector a thread.  Against a block per row (above) there is always something on the way, and
  * what does not depend on the row (gamma, addresses) is done once: the instructions of 16-bit rows bound that
- * kernel (43 an element, 73 % of the issue slots). */
+ * kernel (43 an element, 73 % of the issue slots).
+ * Two blocks to an SM, each two rows ahead: 51.5 us for 8192 x 4096 with the sum, the plain and the fp8 output (5.9 TB/s); four rows
+ * ahead 52.5, three blocks 56, and compiled for the registers of two blocks 64, with the same counts of
+ * instructions: reads and writes share the memory best when neither runs far ahead. */
 template <typename T>
-__global__ void __launch_bounds__(512, 2)
+__global__ void __launch_bounds__(512, 3)
 decxb_rmsnorm_rows_kernel(const NormArgs a, const int stages, const long long wait_limit_ns, decxb_dev_status* status)
 {
     extern __shared__ __align__(128) uint8_t smem[];
@@ -287,11 +290,11 @@ template <typename T>
 int launch_norm_many(decxb_ctx* ctx, const NormArgs& a, cudaStream_t s)
 {
     auto kernel = decxb_rmsnorm_rows_kernel<T>;
-    const int stages = 4;
-    const size_t smem = (size_t)stages * a.cols * sizeof(T) * (a.r ? 2 : 1);      /* at most 64 KiB */
+    const int stages = 2;
+    const size_t smem = (size_t)stages * a.cols * sizeof(T) * (a.r ? 2 : 1);      /* at most 32 KiB */
     static std::once_flag once[DECXB_MAX_DEVICES];
     static cudaError_t err[DECXB_MAX_DEVICES];
-    std::call_once(once[ctx->device], [&] { err[ctx->device] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024); });
+    std::call_once(once[ctx->device], [&] { err[ctx->device] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 32 * 1024); });
     if (err[ctx->device] != cudaSuccess) return decxb_fail(ctx, DECXB_ERR_CUDA, std::string("norm kernel attributes: ") + cudaGetErrorString(err[ctx->device]));
     return launch_after(ctx, kernel, (unsigned)(2 * ctx->sm_count), threads_for(decxb_ceil_div(a.cols, 8), 1, 512), smem, s, a, stages,
                         ctx->wait_limit_ns, ctx->d_status);
@@ -303,7 +306,7 @@ template <typename T>
 int launch_norm(decxb_ctx* ctx, const NormArgs& a, cudaStream_t s)
 {
     const int64_t nvec = decxb_ceil_div(a.cols, 8);
-    /* 16-bit rows of 2049 to 4096 columns, eight or more to an SM: 8192 x 4096 60.6 us with a block a row, 51.8 with rows by bulk
+    /* 16-bit rows of 2049 to 4096 columns, eight or more to an SM: 8192 x 4096 60.6 us with a block a row, 51.5 with rows by bulk
      * copies; but 600 x 4096 5.6 and 7.0, 16384 x 1024 29 and 58, 4096 x 4096 fp32 46.6 and 53.8 */
     if constexpr (sizeof(T) == 2)
         if (a.vec && a.gvec && a.cols % 8 == 0 && (!a.q || a.qvec) && a.cols > 2048 && a.cols <= 4096 && a.rows >= 8 * (int64_t)ctx->sm_count)
@@ -614,13 +617,23 @@ decxb_quantize_fp8_kernel(const QuantArgs a)
     const int64_t row = r0 + g * 8, col = c0 + t * 8;
     const int nr = (int)max((int64_t)0, min((int64_t)8, a.rows - row));          /* rows and columns that exist here */
     const int nc = (int)max((int64_t)0, min((int64_t)8, a.cols - col));
+    /* all 128 columns there, every row a vector of its own: one question a row (11 integer instructions an element otherwise) */
+    const bool full = c0 + 128 <= a.cols;
     start_after_previous();
     Raw8<T> x[8];
+    const T* px = static_cast<const T*>(a.x) + row * a.ldx + col;
+    if (full && a.vec) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) load_raw(static_cast<const T*>(a.x) + (row + i) * a.ldx + col, i < nr ? nc : 0, a.vec, x[i]);
+        for (int i = 0; i < 8; ++i, px += a.ldx)
+#pragma unroll
+            for (int k = 0; k < (int)sizeof(T) / 2; ++k) x[i].u[k] = i < nr ? *(reinterpret_cast<const uint4*>(px) + k) : make_uint4(0, 0, 0, 0);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i, px += a.ldx) load_raw(px, i < nr ? nc : 0, a.vec, x[i]);
+    }
     auto word = [&](int i, int k) { return reinterpret_cast<const uint32_t*>(x[i].u)[k]; };
     auto lane_of = [&](uint32_t w, int e) -> float {      /* column e of a word */
-        if constexpr (E == 2) { const T* p = reinterpret_cast<const T*>(&w); return to_f32(p[e]); }
+        if constexpr (E == 2) { float f, g; halves(w, kind, f, g); return e ? g : f; }
         else return __uint_as_float(w);
     };
 
@@ -692,15 +705,19 @@ decxb_quantize_fp8_kernel(const QuantArgs a)
         }
         Quantiser z = quantiser(s);
         const float s_row = z.minus_s, inv_row = z.inv;
+        uint8_t* q = a.q.data + row * a.q.ld + col;
+        const bool fast = full && a.q.vec;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 8; ++i, q += a.q.ld) {
             if (a.q.block_rows == 1) {
                 z.minus_s = __shfl_sync(0xffffffffu, s_row, 2 * i, 16);
                 z.inv = __shfl_sync(0xffffffffu, inv_row, 2 * i, 16);
             }
             float v[8];
             unpack(x[i], v);
-            if (i < nr && nc > 0) store_codes8(a.q.data + (row + i) * a.q.ld + col, nc, a.q.vec, codes8<TYPE>(v, z));
+            const uint2 c = codes8<TYPE>(v, z);
+            if (fast) { if (i < nr) *reinterpret_cast<uint2*>(q) = c; }
+            else if (i < nr && nc > 0) store_codes8(q, nc, a.q.vec, c);
         }
     }
 
@@ -720,11 +737,14 @@ decxb_quantize_fp8_kernel(const QuantArgs a)
         __syncthreads();
         /* out: row c of the transpose, eight of X's rows per thread, 16 lanes a row */
         const int nro = (int)max((int64_t)0, min((int64_t)8, a.rows - (r0 + t * 8)));
+        uint8_t* o = a.t.data + (c0 + g) * a.t.ld + r0 + t * 8;
+        const bool fast = full && a.t.vec && nro == 8;
 #pragma unroll
-        for (int p = 0; p < 8; ++p) {
+        for (int p = 0; p < 8; ++p, o += 16 * a.t.ld) {
             const int c = p * 16 + g;
             const uint2 k = *reinterpret_cast<const uint2*>(tr + c * 128 + ((t ^ (c >> 3)) << 3));
-            if (c0 + c < a.cols && nro > 0) store_codes8(a.t.data + (c0 + c) * a.t.ld + r0 + t * 8, nro, a.t.vec, k);
+            if (fast) *reinterpret_cast<uint2*>(o) = k;
+            else if (c0 + c < a.cols && nro > 0) store_codes8(o, nro, a.t.vec, k);
         }
     }
 }
