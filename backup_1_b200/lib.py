@@ -216,13 +216,20 @@ def _stream(stream):
     return stream.cuda_stream or 1
 
 
+def _device_ptr(x):
+    """Address of an argument that has to be in device memory: a tensor or a raw address, not an array of the host."""
+    if hasattr(x, "ctypes"):
+        raise TypeError("a numpy array is in host memory")
+    return _ptr(x)
+
+
 class Fp8Matrix:
     """An fp8 matrix with a scale for each block of block_rows x 128 codes (decxb_fp8_matrix): codes [rows][cols] with
     row pitch `ld`, scale of element (r, c) at (r // block_rows) * scale_row_stride + (c // 128) * scale_block_stride."""
 
     def __init__(self, data, scales, rows, cols, ld, scale_row_stride, scale_block_stride, block_rows=1, type=FP8_E4M3):
         self.data, self.scales = data, scales          # kept alive with the descriptor
-        self.c = Fp8MatrixStruct(_ptr(data), _ptr(scales), rows, cols, ld, scale_row_stride, scale_block_stride, type, block_rows)
+        self.c = Fp8MatrixStruct(_device_ptr(data), _device_ptr(scales), rows, cols, ld, scale_row_stride, scale_block_stride, type, block_rows)
         self.addr = C.addressof(self.c)
         self.rows, self.cols, self.block_rows, self.type = rows, cols, block_rows, type
         on = {t.get_device() for t in (data, scales) if hasattr(t, "get_device")}
@@ -410,7 +417,7 @@ class Context:
             _dtype(x, element)
         if hasattr(x, "get_device") and x.get_device() != self.device:
             raise DecxbError(13, f"a tensor on {x.device} was passed to a context of cuda:{self.device}")
-        return _ptr(x)
+        return _device_ptr(x)
 
     def _fp8(self, m):
         """Address of an fp8 matrix argument's descriptor."""

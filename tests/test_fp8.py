@@ -61,6 +61,8 @@ def test_descriptor_from_tensors():
     for data, scales in [(code.float(), torch.empty((5, 3))), (code, torch.empty((5, 3), dtype=torch.float64))]:
         with pytest.raises(TypeError):
             b.Fp8Matrix.of(data, scales)
+    with pytest.raises(TypeError):                      # host memory
+        b.Fp8Matrix(torch.zeros(16, 16).numpy(), 4096, 16, 16, 16, 1, 16)
 
 
 def test_stream_argument():
@@ -141,7 +143,8 @@ def test_product_types_addend_and_results_pitch(ctx, M, N, K, dtype, kinds):
 @gpu
 @pytest.mark.parametrize("b_rows", [1, 128])
 @pytest.mark.parametrize("dtype", FLOATS)
-@pytest.mark.parametrize("M,N,K,pad", [(2055, 1288, 384, 0), (2055, 1288, 300, 1), (2304, 1283, 130, 5), (40, 20000, 260, 8)])
+@pytest.mark.parametrize("M,N,K,pad", [(2055, 1288, 384, 0), (2055, 1288, 300, 1), (2304, 1283, 130, 5), (40, 20000, 260, 8), (5000, 4200, 640, 0),
+                                       (4999, 4101, 390, 3)])
 def test_product_of_many_tiles_with_addend(ctx, M, N, K, pad, dtype, b_rows):
     """Addend and result through the copy engine (pitch and N of whole 16-byte pieces) and by the threads, in place too."""
     g = gen(K)
@@ -610,6 +613,9 @@ def test_norm_refusals(ctx):
     bad(13, R=torch.zeros((4, 256)), ldr=256)
     with pytest.raises(TypeError):
         ctx.rmsnorm(4, 256, x, 256, gamma, 1e-6, Y=y.half(), ldy=256)
+    with pytest.raises(TypeError):
+        ctx.rmsnorm(4, 256, x.cpu().numpy(), 256, gamma, 1e-6, Y=y, ldy=256)
+    bad(13, X=x.cpu())
 
     def badb(status, rows=4, dX=y, lddx=256, **kw):
         with pytest.raises(b.DecxbError) as e:
