@@ -609,7 +609,7 @@ decxb_quantize_fp8_kernel(const QuantArgs a)
     const T* const kind = nullptr;
     __shared__ uint32_t colmax[8][16 * W];
     __shared__ uint32_t wmax[8];
-    __shared__ float colscale[128];
+    __shared__ __align__(16) Quantiser colq[128];
     __shared__ __align__(16) uint8_t tr[128 * 128];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = tid >> 4, t = tid & 15;
     const int64_t tile_r = blockIdx.x / a.tiles_c, tile_c = blockIdx.x % a.tiles_c;
@@ -671,7 +671,7 @@ decxb_quantize_fp8_kernel(const QuantArgs a)
         for (int w = 1; w < 8; ++w) m = max_word(m, colmax[w][tid / E], kind);
         const float s = scale_of(lane_of(m, tid % E), TYPE, a.rule);
         if (c0 + tid < a.cols) a.t.s[(c0 + tid) * a.t.srs + tile_r * a.t.sbs] = s;
-        colscale[tid] = s;
+        colq[tid] = quantiser(s);
     }
 
     if (a.q.data) {
@@ -728,7 +728,7 @@ decxb_quantize_fp8_kernel(const QuantArgs a)
         Quantiser z = quantiser(st);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            if (by_col) z = quantiser(colscale[t * 8 + j]);
+            if (by_col) z = colq[t * 8 + j];
             float v[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = lane_of(word(i, j / E), j % E);
