@@ -150,10 +150,23 @@ __device__ __forceinline__ float scale_of(float amax, int type, int rule)
  * the rounding of s itself, so a product with 1 / s alone, one step of fp32 off, turns four codes in ten thousand
  * over: one correction by the remainder x - q s makes it the fp32 quotient.  (With the power-of-two rule the product is
  * exact and the remainder 0.) */
-struct Quantiser { float inv, minus_s; };    /* 1 / scale, and -scale (0 for an infinite one, whose finite values give 0) */
+struct alignas(8) Quantiser { float inv, minus_s; };    /* 1 / scale, and -scale (0 for an infinite one, whose finite values give 0) */
 __device__ __forceinline__ Quantiser quantiser(float scale)
 {
     return Quantiser{__frcp_rn(scale), scale < INFINITY ? -scale : 0.0f};
+}
+
+template <int TYPE>
+__device__ __forceinline__ uint32_t codes4(const float* f)
+{
+    uint32_t r;
+    if constexpr (TYPE == DECXB_FP8_E4M3)
+        asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\tmov.b32 %0, {lo, hi};\n\t}"
+            : "=r"(r) : "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]));
+    else
+        asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e5m2x2.f32 lo, %2, %1;\n\tcvt.rn.satfinite.e5m2x2.f32 hi, %4, %3;\n\tmov.b32 %0, {lo, hi};\n\t}"
+            : "=r"(r) : "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]));
+    return r;
 }
 
 /* Eight codes, rounded to nearest even; saturation only meets what the scale's own rounding pushed a hair over the
@@ -162,15 +175,13 @@ template <int TYPE>
 __device__ __forceinline__ uint2 codes8(const float* v, const Quantiser& z)
 {
     const uint64_t inv = pack2(z.inv, z.inv), s = pack2(z.minus_s, z.minus_s);
-    uint32_t h[4];
+    float f[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const uint64_t x = pack2(v[2 * j], v[2 * j + 1]), q = mul2(x, inv);
-        float a, b;
-        unpack2(fma2(fma2(q, s, x), inv, q), a, b);
-        h[j] = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, TYPE == DECXB_FP8_E4M3 ? __NV_E4M3 : __NV_E5M2);
+    for (int j = 0; j < 8; j += 2) {
+        const uint64_t x = pack2(v[j], v[j + 1]), q = mul2(x, inv);
+        unpack2(fma2(fma2(q, s, x), inv, q), f[j], f[j + 1]);
     }
-    return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+    return make_uint2(codes4<TYPE>(f), codes4<TYPE>(f + 4));
 }
 
 __device__ __forceinline__ void store_codes8(uint8_t* p, int n, bool vec, uint2 c)

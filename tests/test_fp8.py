@@ -343,6 +343,35 @@ def test_quantise_orientations_of_different_types(ctx):
 
 
 @gpu
+@pytest.mark.parametrize("blocks", [(1, 1), (128, 128), (1, 128), (128, 1)])
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_quantise_special_values_in_every_row_and_column_of_a_tile(ctx, dtype, blocks):
+    """Blocks that hold a NaN or an infinity, wherever it lies and whatever its sign, next to blocks that hold none; the
+    second row of tiles and the last column of tiles are cut."""
+    rows, cols = 200, 600
+    g = gen(9)
+    x = torch.randn(rows, cols, device=DEV, generator=g).to(dtype)
+    x[torch.arange(0, 128, 2), torch.arange(0, 128, 2)] = float("nan")          # tile 0: every other row and column
+    x[torch.arange(0, 64), 128 + torch.arange(64, 128)] = -float("inf")         # tile 1: the upper rows, the last columns
+    x[torch.arange(128, 200), 256 + torch.arange(0, 72)] = -float("nan")        # a cut tile
+    x[:, 384:512] = -x[:, 384:512].abs()                                        # the largest magnitude is negative
+    x[199, 599] = float("inf")
+    Q, T = b.Fp8Matrix.empty(rows, cols, blocks[0]), b.Fp8Matrix.empty(cols, rows, blocks[1])
+    ctx.quantize_fp8(rows, cols, x, cols, Q, T, stream=cur())
+    ctx.synchronize()
+    for m, y, blk in ((Q, x.double(), blocks[0]), (T, x.double().t(), blocks[1])):
+        amax = blocks_amax(y, blk)
+        want = torch.where(torch.isfinite(amax), want_scales(amax.nan_to_num(1.0, 1.0), m.type, b.SCALE_AMAX).double(), amax).float()
+        assert torch.equal(m.scales.nan_to_num(-1.0, -2.0), want.nan_to_num(-1.0, -2.0))
+        scale, code = spread(want, blk, *y.shape).double(), m.data.double()
+        none = torch.isnan(scale) | torch.isinf(y)
+        assert torch.equal(torch.isnan(code), none)
+        assert bool((code[torch.isinf(scale) & ~none] == 0).all())
+        ok = torch.isfinite(scale)
+        check_codes(m.data[ok], y[ok] / scale[ok], m.type, 0.0)
+
+
+@gpu
 def test_quantise_zeros_nan_infinity_and_tiny(ctx):
     x = torch.randn(6, 256, device=DEV)
     x[0] = 0.0
