@@ -126,12 +126,16 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar)
 {
     asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory");
 }
-/* Arrival on the leader CTA's barrier.  What it releases are reads of tensor memory, which tcgen05.wait::ld and the
- * tcgen05 fence before it have ordered; a release at cluster scope would add a memory fence of about a thousand
- * clocks, twice a k-block's arithmetic. */
-__device__ __forceinline__ void mbar_arrive_leader(uint32_t bar)
+/* One elected lane of a converged warp arrives on a barrier of the cluster and on one of its own CTA.  What the first releases are
+ * reads of tensor memory, which tcgen05.wait::ld and the tcgen05 fence before it have ordered; a release at cluster scope would add
+ * a memory fence of about a thousand clocks, twice a k-block's arithmetic.  Both CTAs of a pair address the leader's barrier the same
+ * way and the lane is chosen by a predicate: with branches for either the warp's next wait began later, and 4096 x 4096 x 8192
+ * took 184 us (a factor per row) and 129 (one per block), so 164 and 122. */
+__device__ __forceinline__ void mbar_arrive_both(uint32_t bar_cluster, uint32_t bar)
 {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" :: "r"(mapa(bar, 0)) : "memory");
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\t"
+                 "@p mbarrier.arrive.shared::cluster.b64 _, [%0];\n\t"
+                 "@p mbarrier.arrive.release.cta.shared::cta.b64 _, [%1];\n\t}" :: "r"(bar_cluster), "r"(bar) : "memory");
 }
 
 __device__ __forceinline__ float lds_f32(uint32_t at)
@@ -294,14 +298,15 @@ __device__ __forceinline__ void put4(const Params& p, int64_t row, int64_t col, 
 
 /* --------------------------------------------------------------------------------------
  * Many result tiles: a pair of CTAs (cta_group::2) per tile of 256 x 256, each with 128 rows of A and 128 of B.
- * 16384 x 4096 x 8192 takes 550 us (2.0 PFLOP/s, the SM clock near 1.55 GHz under the power cap). A k-block costs 930
+ * 16384 x 4096 x 8192 takes 480 to 530 us (2.1 to 2.3 PFLOP/s, the SM clock near 1.55 GHz under the power cap). A k-block costs 880
  * clocks of an SM where the tensor core needs 512: feeding the tiles alone takes 231 us of that size, the MMAs alone
  * about 440, reading tensor memory and adding alone 393, and the last two overlap only in part, two accumulators being
- * all that tensor memory holds. With a factor per column two multiplications an element bound it: 1.46 PFLOP/s.
+ * all that tensor memory holds. With a factor per column two operations an element, and what the
+ * same warps wait between k-blocks, bound it: 1.67 PFLOP/s.
  * COLVEC : B has a scale per row (block_rows 1): each column of the tile has its own factor.  Otherwise a
  *          128-row block of B has one scale, and the columns of one epilogue warp lie in one block.
  * ADDEND : C comes through the copy engine into the boxes that the results leave from, the first of a tile during its
- *          product (4096 x 4096 x 8192 with an fp32 addend: 222 us, with the threads' own loads 436).
+ *          product (4096 x 4096 x 8192 with an fp32 addend: 218 us, with the threads' own loads 436).
  * ------------------------------------------------------------------------------------ */
 template <bool COLVEC>
 struct Cfg {
@@ -491,6 +496,7 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
             mbar_arrive_expect_tx(bar, 4096);
             tma_load_2d(box0 + (uint32_t)(i & 1) * 4096u, &map_c, bar, (int)col, (int)row);
         };
+        const uint32_t tempty_at = mapa(tempty_bar(0), 0);      /* the leader's */
         int unit = 0, slot = 0, stage = 0;
         uint32_t sphase = 0, phase = 0;
         bool alive = true;
@@ -539,7 +545,7 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                     tmem_ld_wait_n<32>(w);
                     if (c + 32 < C::ACC) load32(c + 32, v[((c >> 5) + 1) & 1]);
                     if constexpr (COLVEC) {
-                        /* (two numbers an instruction: 4096 x 4096 x 8192 188 us, with one 205) */
+                        /* (two numbers an instruction save 8 % of 4096 x 4096 x 8192) */
 #pragma unroll
                         for (int g = 0; g < 4; ++g) {
                             const uint64_t x = lds_b64(sc + (uint32_t)(BM_CTA + eh * C::ACC + c + g * 8 + (lane & 3) * 2) * 4u);
@@ -557,12 +563,7 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                 /* block taken: hand the buffer (in the leader CTA) and the scales' slot back */
                 tc_fence_before();
                 __syncwarp();
-                if (elect_one()) {
-                    if (is_leader) mbar_arrive(tempty_bar(acc));
-                    else           mbar_arrive_leader(tempty_bar(acc));
-                    mbar_arrive(sempty_bar(slot));
-                }
-                __syncwarp();
+                mbar_arrive_both(tempty_at + 8u * (uint32_t)acc, sempty_bar(slot));
                 if (++slot == SLOTS) { slot = 0; sphase ^= 1u; }
                 if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
             }
