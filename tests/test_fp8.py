@@ -809,6 +809,26 @@ def test_pitches_and_offsets_beyond_32_bits(ctx):
     assert torch.equal(torch.as_strided(dist, (rows, 256), (far, 1)), (near.float() * 2).bfloat16())
 
 
+@gpu
+@pytest.mark.parametrize("short", [16, 0])
+def test_quantise_rows_up_to_and_over_16_mib_apart(ctx, short):
+    """Whole tiles whose rows lie just under 2^24 bytes apart, and just there, in the input and in both outputs."""
+    rows, cols, apart = 128, 256, 2 ** 24 - short
+    g = gen(6)
+    x = torch.randn(rows, cols, device=DEV, generator=g).to(torch.bfloat16)
+    far = torch.empty(rows * apart // 2, device=DEV, dtype=torch.bfloat16)
+    torch.as_strided(far, (rows, cols), (apart // 2, 1)).copy_(x)
+    q, t = (torch.empty(n * apart, device=DEV, dtype=torch.float8_e4m3fn) for n in (rows, cols))
+    Q = b.Fp8Matrix.of(torch.as_strided(q, (rows, cols), (apart, 1)), torch.empty(rows, 2, device=DEV))
+    T = b.Fp8Matrix.of(torch.as_strided(t, (cols, rows), (apart, 1)), torch.empty(cols, 1, device=DEV))
+    nearQ, nearT = b.Fp8Matrix.empty(rows, cols), b.Fp8Matrix.empty(cols, rows)
+    ctx.quantize_fp8(rows, cols, far, apart // 2, Q, T, stream=cur())
+    ctx.quantize_fp8(rows, cols, x, cols, nearQ, nearT, stream=cur())
+    ctx.synchronize()
+    for a, c in ((Q, nearQ), (T, nearT)):
+        assert torch.equal(a.data.view(torch.uint8), c.data.view(torch.uint8)) and torch.equal(a.scales, c.scales)
+
+
 _FIRST_CALL_CAPTURED = r"""
 import torch
 import backup_1_b200 as b
