@@ -126,6 +126,7 @@ struct decxb_ctx {
     int tile_group = 8;                 /* tile-rows per group of the GEMM kernel's tile order (decxb_set_tile_group) */
     int reserved_sms = 0;               /* SMs the next GEMM launches leave free (a transfer kernel runs beside them) */
     int inject_countdown = -1;          /* >= 0: that many pipeline CUDA calls from now, one reports a failure (tests) */
+    std::atomic<int64_t> lost_copy{-1}; /* >= 0: the next launch that waits for copies leaves this row's or tile's out (tests) */
     std::string last_error;
     /* per-kernel event timing (decxb_profile_*) */
     bool profiling = false;

@@ -118,6 +118,13 @@ extern "C" int decxb_set_wait_limit_ms(decxb_ctx* ctx, int ms)
     return DECXB_OK;
 }
 
+extern "C" int decxb_inject_lost_copy(decxb_ctx* ctx, int64_t row_or_tile)
+{
+    if (!ctx) return DECXB_ERR_BAD_PARAM;
+    ctx->lost_copy = row_or_tile < 0 ? -1 : row_or_tile;
+    return DECXB_OK;
+}
+
 extern "C" int decxb_set_tile_group(decxb_ctx* ctx, int tile_rows)
 {
     if (!ctx || tile_rows < 1 || tile_rows > 64) return DECXB_ERR_BAD_PARAM;

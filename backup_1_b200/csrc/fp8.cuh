@@ -257,5 +257,9 @@ inline int refuse_capture(decxb_ctx* ctx, cudaStream_t s, const char* what)
     return DECXB_OK;
 }
 
+/* The row (of a norm) or result tile (of a product) whose copies the next launch that waits for copies leaves out, once
+ * (decxb_inject_lost_copy); -1: none. */
+inline int64_t lost_copy(decxb_ctx* ctx) { return ctx->lost_copy.load(std::memory_order_relaxed) < 0 ? -1 : ctx->lost_copy.exchange(-1); }
+
 }  // namespace fp8
 #endif

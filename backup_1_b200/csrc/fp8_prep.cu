@@ -47,12 +47,14 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                  :: "r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
-/* Wait for a stage's copies; where they do not come within the limit, the status word says so and the wait ends. */
-__device__ __forceinline__ void wait_copy(uint32_t bar, uint32_t parity, long long limit_ns, decxb_dev_status* status)
+/* Wait for a stage's copies.  False where they did not come within the limit, which the status word then says, or where
+ * another wait had given up before. */
+__device__ __forceinline__ bool wait_copy(uint32_t bar, uint32_t parity, long long limit_ns, decxb_dev_status* status)
 {
     unsigned long long t0 = 0;
     for (uint32_t spins = 1; !tcptx::mbar_try_wait(bar, parity); ++spins) {
         if (spins & 1023u) continue;
+        if (*reinterpret_cast<volatile int*>(&status->code) != 0) return false;
         const unsigned long long t = tcptx::globaltimer_ns();
         if (t0 == 0) t0 = t;
         if ((long long)(t - t0) > limit_ns) {
@@ -60,8 +62,19 @@ __device__ __forceinline__ void wait_copy(uint32_t bar, uint32_t parity, long lo
                 status->where = 3000; status->block = (int)blockIdx.x; status->detail = 0;
                 __threadfence_system();
             }
-            return;
+            return false;
         }
+    }
+    return true;
+}
+
+/* By the thread that fetches, when a block leaves its rows early: waits (with a limit) for the copies of `row` and of the
+ * stages behind it, which may still be on their way into the block's shared memory. */
+__device__ __forceinline__ void drain_copies(uint64_t* bars, int stages, int st, uint32_t phase, int64_t row, int64_t rows)
+{
+    for (int i = 0; i < stages && row < rows; ++i, row += gridDim.x) {
+        for (int tries = 0; tries < 2048 && !tcptx::mbar_try_wait(tcptx::smem_u32(&bars[st]), phase); ++tries) __nanosleep(64);
+        if (++st == stages) { st = 0; phase ^= 1u; }
     }
 }
 
@@ -167,10 +180,11 @@ decxb_rmsnorm_kernel(const NormArgs a)
  * instructions: reads and writes share the memory best when neither runs far ahead. */
 template <typename T>
 __global__ void __launch_bounds__(512, 3)
-decxb_rmsnorm_rows_kernel(const NormArgs a, const int stages, const long long wait_limit_ns, decxb_dev_status* status)
+decxb_rmsnorm_rows_kernel(const NormArgs a, const int stages, const long long wait_limit_ns, decxb_dev_status* status, const int64_t lost_row)
 {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float part[2][16];
+    __shared__ int lost[2];                    /* a thread gave its wait up; alternates with `part` */
     __shared__ __align__(8) uint64_t bars[8];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nwarps = blockDim.x >> 5, cols = (int)a.cols;
     const int arrays = a.r ? 2 : 1;
@@ -179,10 +193,12 @@ decxb_rmsnorm_rows_kernel(const NormArgs a, const int stages, const long long wa
     auto fetch = [&](int64_t row, int st) {
         const uint32_t bar = tcptx::smem_u32(&bars[st]), at = tcptx::smem_u32(smem) + (uint32_t)(st * arrays) * row_bytes;
         tcptx::mbar_arrive_expect_tx(bar, row_bytes * arrays);
+        if (row == lost_row) return;
         bulk_load(at, static_cast<const T*>(a.x) + row * a.ldx, row_bytes, bar);
         if (a.r) bulk_load(at + row_bytes, static_cast<const T*>(a.r) + row * a.ldr, row_bytes, bar);
     };
     if (tid == 0) {
+        lost[0] = lost[1] = 0;
         for (int st = 0; st < stages; ++st) tcptx::mbar_init(tcptx::smem_u32(&bars[st]), 1);
         tcptx::fence_barrier_init();
     }
@@ -196,7 +212,7 @@ decxb_rmsnorm_rows_kernel(const NormArgs a, const int stages, const long long wa
     const float of_cols = 1.0f / (float)cols;
     int st = 0, turn = 0; uint32_t phase = 0;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
-        wait_copy(tcptx::smem_u32(&bars[st]), phase, wait_limit_ns, status);
+        if (!wait_copy(tcptx::smem_u32(&bars[st]), phase, wait_limit_ns, status)) lost[turn] = 1;
         const T* in = reinterpret_cast<const T*>(smem + (size_t)(st * arrays) * row_bytes);
         float v[8], sum = 0.0f;
         load8(in + first, n, true, v);
@@ -211,6 +227,10 @@ decxb_rmsnorm_rows_kernel(const NormArgs a, const int stages, const long long wa
         sum = warp_sum(sum);
         if (lane == 0) part[turn][warp] = sum;
         __syncthreads();                       /* every thread has its values: the stage can be filled again */
+        if (lost[turn]) {                      /* the row did not come: it and those behind it stay unwritten */
+            if (tid == 0) drain_copies(bars, stages, st, phase, row, a.rows);
+            return;
+        }
         if (tid == 0 && row + (int64_t)stages * gridDim.x < a.rows) fetch(row + (int64_t)stages * gridDim.x, st);
         const float rstd = rsqrtf(warp_sum(lane < nwarps ? part[turn][lane] : 0.0f) * of_cols + a.eps);
         if (a.h && n) store8(static_cast<T*>(a.h) + row * a.ldh + first, 8, true, v);
@@ -297,7 +317,7 @@ int launch_norm_many(decxb_ctx* ctx, const NormArgs& a, cudaStream_t s)
     std::call_once(once[ctx->device], [&] { err[ctx->device] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 32 * 1024); });
     if (err[ctx->device] != cudaSuccess) return decxb_fail(ctx, DECXB_ERR_CUDA, std::string("norm kernel attributes: ") + cudaGetErrorString(err[ctx->device]));
     return launch_after(ctx, kernel, (unsigned)(2 * ctx->sm_count), threads_for(decxb_ceil_div(a.cols, 8), 1, 512), smem, s, a, stages,
-                        ctx->wait_limit_ns, ctx->d_status);
+                        ctx->wait_limit_ns, ctx->d_status, lost_copy(ctx));
 }
 
 /* One vector a thread as far as 1024 threads reach (8192 x 4096 bf16 with one, two, four: 64, 69, 74 us): a block's loads,
@@ -390,10 +410,11 @@ decxb_rmsnorm_backward_kernel(const NormBwdArgs a)
  * 122 us with loads into registers). */
 template <typename T, int VPT>
 __global__ void __launch_bounds__(512, VPT == 1 ? 2 : 1)
-decxb_rmsnorm_backward_rows_kernel(const NormBwdArgs a, const int stages, const long long wait_limit_ns, decxb_dev_status* status)
+decxb_rmsnorm_backward_rows_kernel(const NormBwdArgs a, const int stages, const long long wait_limit_ns, decxb_dev_status* status, const int64_t lost_row)
 {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float2 buf[2][16];
+    __shared__ int lost[2];                    /* a thread gave its wait up; alternates with `buf` */
     __shared__ __align__(8) uint64_t bars[8];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nwarps = blockDim.x >> 5, cols = (int)a.cols;
     const int arrays = a.dr ? 3 : 2;
@@ -402,11 +423,13 @@ decxb_rmsnorm_backward_rows_kernel(const NormBwdArgs a, const int stages, const 
     auto fetch = [&](int64_t row, int st) {
         const uint32_t bar = tcptx::smem_u32(&bars[st]), at = tcptx::smem_u32(smem) + (uint32_t)(st * arrays) * row_bytes;
         tcptx::mbar_arrive_expect_tx(bar, row_bytes * arrays);
+        if (row == lost_row) return;
         bulk_load(at, static_cast<const T*>(a.dy) + row * a.lddy, row_bytes, bar);
         bulk_load(at + row_bytes, static_cast<const T*>(a.h) + row * a.ldh, row_bytes, bar);
         if (a.dr) bulk_load(at + 2 * row_bytes, static_cast<const T*>(a.dr) + row * a.lddr, row_bytes, bar);
     };
     if (tid == 0) {
+        lost[0] = lost[1] = 0;
         for (int st = 0; st < stages; ++st) tcptx::mbar_init(tcptx::smem_u32(&bars[st]), 1);
         tcptx::fence_barrier_init();
     }
@@ -429,8 +452,7 @@ decxb_rmsnorm_backward_rows_kernel(const NormBwdArgs a, const int stages, const 
     }
     int st = 0, turn = 0; uint32_t phase = 0;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
-        /* (a copy that does not come within the limit is recorded; the rows that it leaves wrong are the caller's to discard) */
-        wait_copy(tcptx::smem_u32(&bars[st]), phase, wait_limit_ns, status);
+        if (!wait_copy(tcptx::smem_u32(&bars[st]), phase, wait_limit_ns, status)) lost[turn] = 1;
         const T* in = reinterpret_cast<const T*>(smem + (size_t)(st * arrays) * row_bytes);
         Raw8<T> rw[VPT], rx[VPT], ro[VPT];
         float sq = 0.0f, dot = 0.0f;
@@ -448,6 +470,10 @@ decxb_rmsnorm_backward_rows_kernel(const NormBwdArgs a, const int stages, const 
         }
         /* behind the barrier in here every thread has its values: the stage can be filled again */
         const float2 s = block_sum2(sq, dot, buf[turn], warp, lane, nwarps);
+        if (lost[turn]) {                      /* the row did not come: it and those behind it stay unwritten and out of dgamma */
+            if (tid == 0) drain_copies(bars, stages, st, phase, row, a.rows);
+            break;
+        }
         if (tid == 0 && row + (int64_t)stages * gridDim.x < a.rows) fetch(row + (int64_t)stages * gridDim.x, st);
         const float r = rsqrtf(s.x / (float)cols + a.eps), k = r * r * (s.y / (float)cols);
 #pragma unroll
@@ -544,7 +570,8 @@ int launch_backward_rows(decxb_ctx* ctx, const NormBwdArgs& a, unsigned grid, in
     static cudaError_t err[DECXB_MAX_DEVICES];
     std::call_once(once[ctx->device], [&] { err[ctx->device] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024); });
     if (err[ctx->device] != cudaSuccess) return decxb_fail(ctx, DECXB_ERR_CUDA, std::string("norm kernel attributes: ") + cudaGetErrorString(err[ctx->device]));
-    return launch_after(ctx, kernel, grid, threads_for(decxb_ceil_div(a.cols, 8), VPT, 512), smem, s, a, stages, ctx->wait_limit_ns, ctx->d_status);
+    return launch_after(ctx, kernel, grid, threads_for(decxb_ceil_div(a.cols, 8), VPT, 512), smem, s, a, stages, ctx->wait_limit_ns, ctx->d_status,
+                        lost_copy(ctx));
 }
 
 template <typename T>

@@ -115,6 +115,7 @@ SIGNATURES = {
     "decxb_profile_enable": (_i, [_vp, _i]),
     "decxb_profile_read": (_i, [_vp, C.POINTER(Profile)]),
     "decxb_inject_pipeline_error": (_i, [_vp, _i]),
+    "decxb_inject_lost_copy": (_i, [_vp, _i64]),
     "decxb_gemm_prepare_b": (_i, [_vp, _i, _i64, _i64, _vp, _i64, _vp, C.POINTER(_vp)]),
     "decxb_gemm_f32_prepared": (_i, [_vp, _i, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _i, _vp, _i64, _vp]),
     "decxb_gemm_release_b": (_i, [_vp, _vp, _vp]),

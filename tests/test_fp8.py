@@ -934,3 +934,118 @@ def test_calls_on_the_contexts_own_stream_and_on_another(ctx):
     s.synchronize()
     assert torch.equal(first, again)
     assert math.isfinite(float(again.float().sum()))
+
+
+# ---- borders of the scales' rules ---------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("kind", [b.FP8_E4M3, b.FP8_E5M2])
+@pytest.mark.parametrize("dtype", FLOATS)
+def test_quantise_scales_at_and_next_to_powers_of_two(ctx, dtype, kind):
+    """Blocks whose largest magnitude is the type's largest value times a power of two, and the numbers just under and just over:
+    amax / FMAX is a power of two itself, where a rule by logarithms is off by a factor of two if the logarithm is a step too large."""
+    lo, hi = {torch.bfloat16: (-100, 100), torch.float32: (-100, 100), torch.float16: (-20, 0)}[dtype]
+    at = FMAX[kind] * torch.exp2(torch.arange(lo, hi + 1, device=DEV, dtype=torch.float64))
+    step = 2 * HALF[dtype]                                   # to the next number up, relative to the power of two below
+    amax = torch.cat([at, at * (1 - step / 1.75), at * (1 + step / 1.75)]).to(dtype)      # 448 = 1.75 * 2^8, 57344 = 1.75 * 2^15
+    amax = torch.cat([amax[:2 * at.numel()], amax[2 * at.numel():][torch.isfinite(amax[2 * at.numel():])]])
+    rows = amax.numel()
+    assert torch.unique(amax).numel() == rows
+    g = gen(12)
+    x = (amax[:, None].double() * (2 * torch.rand(rows, 128, device=DEV, generator=g) - 1).double() * 0.99).to(dtype)
+    x[torch.arange(rows), torch.randint(0, 128, (rows,), device=DEV, generator=g)] = amax
+    x[::2] = -x[::2]
+    for rule in (b.SCALE_AMAX, b.SCALE_POW2):
+        Q, T = b.Fp8Matrix.empty(rows, 128, 1, kind), b.Fp8Matrix.empty(128, rows, 1, kind)
+        ctx.quantize_fp8(rows, 128, x, 128, Q, T, rule=rule, stream=cur())
+        ctx.synchronize()
+        for m, y in ((Q, x.double()), (T, x.double().t())):
+            s = want_scales(blocks_amax(y, 1), kind, rule)
+            assert torch.equal(m.scales, s)
+            check_codes(m.data, (y / spread(s, 1, *y.shape).double()).float().double(), kind, 0.0)
+
+
+# ---- copies that never come ---------------------------------------------------------------------------------------------
+class LostCopy:
+    """Within it the next launch leaves out the copies of one row or tile; on leaving, the wait for them has run out and was reported."""
+
+    def __init__(self, ctx, which):
+        self.ctx, self.which = ctx, which
+
+    def __enter__(self):
+        self.ctx.set_wait_limit_ms(30)
+        assert self.ctx.L.decxb_inject_lost_copy(self.ctx.h, self.which) == 0
+
+    def __exit__(self, kind, *_):
+        self.ctx.L.decxb_inject_lost_copy(self.ctx.h, -1)
+        if kind is None:
+            with pytest.raises(b.DecxbError) as e:
+                self.ctx.synchronize()
+            assert e.value.status == 103
+        self.ctx.set_wait_limit_ms(1000)
+
+
+def sms():
+    return torch.cuda.get_device_properties(0).multi_processor_count
+
+
+@gpu
+@pytest.mark.parametrize("turn", [0, 2, 3])
+@pytest.mark.parametrize("res", [False, True])
+def test_norm_leaves_rows_that_did_not_come(ctx, turn, res):
+    """A block's row of its first, third or fourth turn does not come: that row and the block's later ones stay as they were, all others are right."""
+    cols, grid = 2304, 2 * sms()
+    rows = 6 * grid + 11
+    g = gen(31)
+    x, r = (torch.randn(rows, cols, device=DEV, generator=g).bfloat16() for _ in range(2))
+    gamma = torch.randn(cols, device=DEV, generator=g)
+    kw = dict(R=r, ldr=cols) if res else {}
+
+    def run():
+        Y, Q = torch.full_like(x, 9.0), b.Fp8Matrix.empty(rows, cols)
+        Q.data.view(torch.uint8).fill_(0x11)
+        Q.scales.fill_(7.0)
+        ctx.rmsnorm(rows, cols, x, cols, gamma, 1e-5, Y=Y, ldy=cols, Q=Q, stream=cur(), **kw)
+        torch.cuda.synchronize()
+        return Y, Q.data.view(torch.uint8).clone(), Q.scales.clone()
+    want = run()
+    ctx.synchronize()
+    with LostCopy(ctx, turn * grid + 5):
+        got = run()
+    left = torch.zeros(rows, dtype=torch.bool, device=DEV)
+    left[torch.arange(turn * grid + 5, rows, grid)] = True
+    for v, w, was in zip(got, want, (9.0, 0x11, 7.0)):
+        assert torch.equal(v[~left], w[~left]) and bool((v[left] == was).all())
+    for v, w in zip(run(), want):
+        assert torch.equal(v, w)
+    ctx.synchronize()
+
+
+@gpu
+@pytest.mark.parametrize("turn", [0, 3])
+@pytest.mark.parametrize("cols,dtype", [(1032, torch.bfloat16), (4096, torch.bfloat16), (5120, torch.float16), (9008, torch.bfloat16), (2048, torch.float32)])
+def test_norm_backward_leaves_rows_that_did_not_come(ctx, cols, dtype, turn):
+    grid = ctx.rmsnorm_backward_workspace(2 ** 20, cols) // (4 * cols)          # what the device takes at once
+    rows = 5 * grid + 3
+    g = gen(32)
+    h, dy, dr = (torch.randn(rows, cols, device=DEV, generator=g).to(dtype) for _ in range(3))
+    gamma = torch.randn(cols, device=DEV, generator=g)
+    ws = torch.empty(ctx.rmsnorm_backward_workspace(rows, cols), device=DEV, dtype=torch.uint8)
+
+    def run():
+        dx, dg = torch.full_like(h, 9.0), torch.empty(cols, device=DEV)
+        ctx.rmsnorm_backward(rows, cols, dy, cols, h, cols, gamma, 1e-5, dx, cols, dg, dR=dr, lddr=cols, workspace=ws, workspace_bytes=ws.numel(), stream=cur())
+        torch.cuda.synchronize()
+        return dx, dg
+    want, dgamma = run()
+    ctx.synchronize()
+    with LostCopy(ctx, turn * grid + 2):
+        got, dgamma_without = run()
+    left = torch.zeros(rows, dtype=torch.bool, device=DEV)
+    left[torch.arange(turn * grid + 2, rows, grid)] = True
+    assert torch.equal(got[~left], want[~left]) and bool((got[left] == 9).all())
+    wg, mg = backward_ref(dy[~left], h[~left], gamma, 1e-5, None)[1::2]
+    longest = 6 + -(-grid // 32) + 6                       # as in test_norm_backward
+    assert bool(((dgamma_without.double() - wg).abs() <= (96 + longest + 4) * U * mg).all())
+    again, dg = run()
+    assert torch.equal(again, want) and torch.equal(dg, dgamma)
+    ctx.synchronize()
