@@ -54,6 +54,7 @@ struct Params {
     int d_type;
     bool tma_store;                /* D leaves, and C comes, through the copy engine   */
     bool d_vec;                    /* four results of a row may leave in one store      */
+    int lost_tile;                 /* tile whose last k-block is never brought (tests; -1: none) */
     long long wait_limit_ns;
     decxb_dev_status* status;
 };
@@ -90,6 +91,13 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const P
         }
     }
     return true;
+}
+
+/* When the issuer leaves early: waits (with a limit) for the commit of its last k-block, whose matrix instructions may still be at work
+ * on tensor memory that is about to be given back. */
+__device__ __forceinline__ void drain_mma(uint32_t bar, uint32_t parity)
+{
+    for (int tries = 0; tries < 2048 && !mbar_try_wait(bar, parity); ++tries) __nanosleep(64);
 }
 
 /* A k-block: four steps of 32 codes (two units of 16 bytes in a descriptor), the first overwriting the accumulator, and the commit, by
@@ -145,6 +153,12 @@ __device__ __forceinline__ void mbar_arrive_both(uint32_t bar_cluster, uint32_t 
                  "@p mbarrier.arrive.release.cta.shared::cta.b64 _, [%1];\n\t}" :: "r"(bar_cluster), "r"(bar) : "memory");
 }
 
+__device__ __forceinline__ void sts_u32(uint32_t at, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" :: "r"(at), "r"(v) : "memory"); }
+/* From the shared memory of a CTA of the cluster (this one's included). */
+__device__ __forceinline__ uint32_t lds_cluster_u32(uint32_t at)
+{
+    uint32_t v; asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory"); return v;
+}
 __device__ __forceinline__ float lds_f32(uint32_t at)
 {
     float v; asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory"); return v;
@@ -408,8 +422,10 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                         /* both CTAs' bytes are counted on the leader's barrier */
                         if (is_leader) mbar_arrive_expect_tx(full_bar(stage), 2 * C::STAGE_BYTES);
                         const uint32_t fb = mapa(full_bar(stage), 0);
-                        tma_load_2d_pair(stage_a(stage), &map_a, fb, kb * BK, row_a);
-                        tma_load_2d_pair(stage_b(stage), &map_b, fb, kb * BK, row_b);
+                        if (t != p.lost_tile || kb + 1 < p.num_kb) {
+                            tma_load_2d_pair(stage_a(stage), &map_a, fb, kb * BK, row_a);
+                            tma_load_2d_pair(stage_b(stage), &map_b, fb, kb * BK, row_b);
+                        }
                     }
                     __syncwarp();
                     armed |= 1u << stage;
@@ -418,13 +434,15 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                 }
             }
             /* a wait gave up somewhere: wait (with a limit) for the copies that are still on their way into
-             * shared memory; the leader's barriers count its peer's as well */
-            if (is_leader && lane == 0 && *reinterpret_cast<volatile int*>(&p.status->code) != 0) {
-                for (int s2 = 0; s2 < C::STAGES; ++s2) {
+             * shared memory; the leader's barriers count its peer's as well, but for a stage that only the peer had filled
+             * again, which the peer gives some time */
+            if (lane == 0 && *reinterpret_cast<volatile int*>(&p.status->code) != 0) {
+                for (int s2 = 0; is_leader && s2 < C::STAGES; ++s2) {
                     if (!((armed >> s2) & 1u)) continue;
                     for (int tries = 0; tries < 2048 && !mbar_try_wait(full_bar(s2), (armed_parity >> s2) & 1u); ++tries)
                         __nanosleep(64);
                 }
+                for (int tries = 0; !is_leader && tries < 2048; ++tries) __nanosleep(64);
             }
         } else if (warp == 1) {
             /* -------------------------------------------------------- MMA issuer ------ */
@@ -442,6 +460,7 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                         if (++stage == C::STAGES) { stage = 0; phase ^= 1u; }
                     }
                 }
+                if (!alive && unit > 0) drain_mma(done_bar(stage ? stage - 1 : C::STAGES - 1), stage ? phase : phase ^ 1u);
             }
         } else if (warp == 2) {
             /* -------------------------------------------------------- scale loader ---- */
@@ -676,6 +695,7 @@ decxb_gemm_fp8_split_kernel(const __grid_constant__ CUtensorMap map_w, const __g
     auto sfull_bar  = [&](int s) { return bars + 8u * (2 * C::MOST_STAGES + C::BUFS + s); };
     auto sempty_bar = [&](int s) { return bars + 8u * (2 * C::MOST_STAGES + C::BUFS + SLOTS + s); };
     const uint32_t tmem_slot = bars + 8u * (2 * C::MOST_STAGES + C::BUFS + 2 * SLOTS);
+    const uint32_t lost = tmem_slot + 4;                                    /* this CTA did not get all of its sums */
     auto stage_w = [&](int s) { return smem_base + s * C::STAGE_BYTES; };
     auto stage_x = [&](int s) { return smem_base + s * C::STAGE_BYTES + C::W_BYTES; };
 
@@ -691,6 +711,7 @@ decxb_gemm_fp8_split_kernel(const __grid_constant__ CUtensorMap map_w, const __g
         for (int b = 0; b < C::BUFS; ++b) mbar_init(tempty_bar(b), EPI_WARPS);
         for (int s = 0; s < SLOTS; ++s) { mbar_init(sfull_bar(s), 32); mbar_init(sempty_bar(s), EPI_WARPS); }
         fence_barrier_init();
+        sts_u32(lost, 0);
     }
     if (warp == 1) {
         tmem_alloc<1>(tmem_slot, C::TMEM_COLS);
@@ -708,6 +729,7 @@ decxb_gemm_fp8_split_kernel(const __grid_constant__ CUtensorMap map_w, const __g
 
     if (warp == 0) {
         /* ------------------------------------------------------------ TMA producer ---- */
+        const int lost_kb = tile == p.lost_tile && rank == 0 ? kb_last - 1 : -1;
         int stage = 0; uint32_t phase = 0;
         uint32_t armed = 0, armed_parity = 0;
         for (int kb = kb_first; kb < kb_last; ++kb) {
@@ -715,8 +737,10 @@ decxb_gemm_fp8_split_kernel(const __grid_constant__ CUtensorMap map_w, const __g
             if (elect_one()) {
                 const uint32_t fb = full_bar(stage);
                 mbar_arrive_expect_tx(fb, C::STAGE_BYTES);
-                tma_load_2d(stage_w(stage), &map_w, fb, kb * BK, n0);
-                tma_load_2d(stage_x(stage), &map_x, fb, kb * BK, m0);
+                if (kb != lost_kb) {
+                    tma_load_2d(stage_w(stage), &map_w, fb, kb * BK, n0);
+                    tma_load_2d(stage_x(stage), &map_x, fb, kb * BK, m0);
+                }
             }
             __syncwarp();
             armed |= 1u << stage;
@@ -734,8 +758,11 @@ decxb_gemm_fp8_split_kernel(const __grid_constant__ CUtensorMap map_w, const __g
         int stage = 0; uint32_t phase = 0;
         for (int unit = 0; unit < kb_last - kb_first; ++unit) {
             const int acc = unit % C::BUFS;
-            if (!warp_wait(full_bar(stage), phase, p, 2300 + stage, tile)) break;
-            if (!warp_wait(tempty_bar(acc), ((uint32_t)(unit / C::BUFS) & 1u) ^ 1u, p, 2200 + acc, tile)) break;
+            if (!warp_wait(full_bar(stage), phase, p, 2300 + stage, tile) ||
+                !warp_wait(tempty_bar(acc), ((uint32_t)(unit / C::BUFS) & 1u) ^ 1u, p, 2200 + acc, tile)) {
+                if (unit > 0) drain_mma(done_bar(stage ? stage - 1 : stages - 1), stage ? phase : phase ^ 1u);
+                break;
+            }
             tc_fence_after();
             umma_block<1>(tmem_base + (uint32_t)(acc * NT), make_smem_desc(stage_w(stage)), make_smem_desc(stage_x(stage)), p.idesc, done_bar(stage));
             if (++stage == stages) { stage = 0; phase ^= 1u; }
@@ -776,14 +803,15 @@ decxb_gemm_fp8_split_kernel(const __grid_constant__ CUtensorMap map_w, const __g
         for (int i = 0; i < C::CW; ++i) sum[i] = 0.0f;
         int stage = 0, slot = 0;
         uint32_t phase = 0, sphase = 0;
+        bool alive = true;
         for (int unit = 0; unit < kb_last - kb_first; ++unit) {
             const int acc = unit % C::BUFS;
-            if (!warp_wait(sfull_bar(slot), sphase, p, 2600 + slot, tile)) break;
+            if (!warp_wait(sfull_bar(slot), sphase, p, 2600 + slot, tile)) { alive = false; break; }
             const uint32_t sc = ring + (uint32_t)(slot * C::KB_FLOATS) * 4u;
             float sw[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) sw[i] = lds_f32(sc + (uint32_t)(q * 32 + i * 8 + (lane >> 2)) * 4u);
-            if (!warp_wait(done_bar(stage), phase, p, 2400 + stage, tile)) break;
+            if (!warp_wait(done_bar(stage), phase, p, 2400 + stage, tile)) { alive = false; break; }
             tc_fence_after();
 #pragma unroll
             for (int c = 0; c < C::CW; c += 8 * G) {
@@ -810,22 +838,31 @@ decxb_gemm_fp8_split_kernel(const __grid_constant__ CUtensorMap map_w, const __g
             if (++slot == SLOTS) { slot = 0; sphase ^= 1u; }
             if (++stage == stages) { stage = 0; phase ^= 1u; }
         }
-        /* every MMA of this CTA has run, so the stages can hold its sums: [token][row of B] */
+        if (alive) {
+            /* every MMA of this CTA has run, so the stages can hold its sums: [token][row of B] */
 #pragma unroll
-        for (int c = 0; c < C::CW; c += 8 * G)
+            for (int c = 0; c < C::CW; c += 8 * G)
 #pragma unroll
-            for (int i = 0; i < 8 * G; ++i) {
-                const int h = i / (4 * G), g = (i / 4) % G, k = i & 3;
-                const int m = eh * C::CW + c + g * 8 + (lane & 3) * 2 + (k & 1), n = q * 32 + h * 16 + (k >> 1) * 8 + (lane >> 2);
-                asm volatile("st.shared.f32 [%0], %1;" :: "r"(smem_base + (uint32_t)(m * C::PITCH + n) * 4u), "f"(sum[c + i]) : "memory");
-            }
+                for (int i = 0; i < 8 * G; ++i) {
+                    const int h = i / (4 * G), g = (i / 4) % G, k = i & 3;
+                    const int m = eh * C::CW + c + g * 8 + (lane & 3) * 2 + (k & 1), n = q * 32 + h * 16 + (k >> 1) * 8 + (lane >> 2);
+                    asm volatile("st.shared.f32 [%0], %1;" :: "r"(smem_base + (uint32_t)(m * C::PITCH + n) * 4u), "f"(sum[c + i]) : "memory");
+                }
+        } else {
+            /* a wait gave up: NaN in place of this warp's sums, which makes those who add them ask, once the copies that are still
+             * on their way into the stages have had their time */
+            for (int tries = 0; tries < 2048; ++tries) __nanosleep(64);
+            for (int m = eh * C::CW; m < (eh + 1) * C::CW; ++m) sts_u32(smem_base + (uint32_t)(m * C::PITCH + q * 32 + lane) * 4u, 0x7fffffffu);
+            if (lane == 0) sts_u32(lost, 1);
+        }
     }
     __syncwarp();
     tc_fence_before();
     if (splits > 1) cluster_sync_all(); else __syncthreads();
 
     /* each CTA finishes its share of the tokens, eight at a time, four columns a thread: the cluster's sums in ascending
-     * order, addend, one rounding */
+     * order, addend, one rounding.  Where a CTA did not get its sums, D stays as it was; the peers' words on that are read only where a
+     * sum is NaN (asked for every tile they cost 1 to 4 %) */
     if (warp >= 4) {
         const int t = (int)threadIdx.x - 128, n = n0 + (t & 31) * 4, rows = (int)min((int64_t)NT, p.M - m0);
         const int have = (int)min((int64_t)4, p.N - n);
@@ -836,6 +873,12 @@ decxb_gemm_fp8_split_kernel(const __grid_constant__ CUtensorMap map_w, const __g
             for (int r = 0; r < splits; ++r) {
                 const float4 w = splits > 1 ? lds_cluster_f32x4(mapa(at, (uint32_t)r)) : lds_f32x4(at);
                 v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+            }
+            if (v.x != v.x) {
+                bool gone = false;
+#pragma unroll 1
+                for (int r = 0; r < splits; ++r) gone |= lds_cluster_u32(mapa(lost, (uint32_t)r)) != 0;
+                if (gone) continue;
             }
             if (p.d_type == DECXB_F32)      put4<float>(p, m0 + m, n, have, v);
             else if (p.d_type == DECXB_F16) put4<__half>(p, m0 + m, n, have, v);
@@ -1088,6 +1131,7 @@ int gemm_fp8(decxb_ctx* ctx, const decxb_fp8_matrix* pa, const decxb_fp8_matrix*
         p.tma_store = aligned(D, ldd * e, 16) && (!C || aligned(C, ldc * e, 16)) && N * e % 16 == 0;
         p.d_vec = aligned(D, ldd * e, 4 * e);
         p.wait_limit_ns = ctx->wait_limit_ns; p.status = ctx->d_status;
+        p.lost_tile = (int)lost_copy(ctx);
         rc = launch_product(ctx, A, B, p, s);
     }
     if (a_copy) decxb_free_on_stream(ctx, a_copy, s);

@@ -517,11 +517,11 @@ DECXB_API int decxb_probe_tensor_peak(decxb_ctx* ctx, int pattern, double target
  * nth_call < 0 switches it off.  Nothing on the device faults.  No counterpart in the reference
  * (its error path prints and exits, srcs/core/error.h:33-42). */
 DECXB_API int decxb_inject_pipeline_error(decxb_ctx* ctx, int nth_call);
-/* Fault injection for tests of the waits on copies: the next launch of a kernel of the 8-bit layer that brings rows to shared
- * memory ahead of their use (decxb_rmsnorm and decxb_rmsnorm_backward on many aligned rows) does not issue the copies of row
- * `row_or_tile`, as if they had been lost.  The wait for them gives up after decxb_set_wait_limit_ms, the row and those that its
- * block would have taken after it are left unwritten, and decxb_synchronize reports DECXB_ERR_TIMEOUT.  One launch;
- * negative: off.  Nothing on the device faults. */
+/* Fault injection for tests of the waits on copies: the next launch of a kernel of the 8-bit layer that brings its operands to shared
+ * memory ahead of their use (decxb_gemm_fp8; decxb_rmsnorm and decxb_rmsnorm_backward on many aligned rows) does not issue the copies of
+ * row `row_or_tile` of a norm, or those of the last k-block of result tile `row_or_tile` of a product, as if they had been lost.  The wait
+ * for them gives up after decxb_set_wait_limit_ms, what its block had still to do is left unwritten, and decxb_synchronize reports
+ * DECXB_ERR_TIMEOUT.  One launch; negative: off.  Nothing on the device faults. */
 DECXB_API int decxb_inject_lost_copy(decxb_ctx* ctx, int64_t row_or_tile);
 
 /* ---- gathering the blocks of a sharded result (NCCL over NVLink) ---------------------------

@@ -1049,3 +1049,45 @@ def test_norm_backward_leaves_rows_that_did_not_come(ctx, cols, dtype, turn):
     again, dg = run()
     assert torch.equal(again, want) and torch.equal(dg, dgamma)
     ctx.synchronize()
+
+
+@gpu
+@pytest.mark.parametrize("M,N,K", [(1, 300, 128), (1, 512, 4096), (20, 700, 2048), (50, 640, 3000), (100, 512, 4096)])
+def test_product_of_few_tiles_leaves_a_tile_that_did_not_come(ctx, M, N, K):
+    """The last k-block of the first share of tile 1 (128 rows of B) does not come: its columns stay as they were, all others are right."""
+    g = gen(33)
+    A, a = int_matrix(g, M, K, b.FP8_E4M3, 1, pad=-K % 16)
+    B, w = int_matrix(g, N, K, b.FP8_E4M3, 128, pad=-K % 16)
+    want = a @ w.t()
+    for tile in (0, 1):
+        D = torch.full((M, N), 9.0, device=DEV)
+        with LostCopy(ctx, tile):
+            ctx.gemm_fp8(A, B, D, N, stream=cur())
+            torch.cuda.synchronize()
+        left = torch.zeros(N, dtype=torch.bool, device=DEV)
+        left[tile * 128:tile * 128 + 128] = True
+        assert torch.equal(D[:, ~left].double(), want[:, ~left]) and bool((D[:, left] == 9).all())
+    assert torch.equal(run_gemm(ctx, A, B, torch.float32).double(), want)
+
+
+@gpu
+@pytest.mark.parametrize("addend", [False, True])
+@pytest.mark.parametrize("b_rows", [1, 128])
+def test_product_of_many_tiles_leaves_tiles_that_did_not_come(ctx, b_rows, addend):
+    """The last k-block of a tile of 256 x 256 does not come: that tile and the later ones of its pair of SMs stay as they were."""
+    M, N, K, pairs = 4096, 4096, 512, sms() // 2
+    g = gen(34)
+    A, a = int_matrix(g, M, K, b.FP8_E4M3, 1)
+    B, w = int_matrix(g, N, K, b.FP8_E4M3, b_rows)
+    Cin = torch.full((M, N), 3.0, device=DEV) if addend else None
+    want = (a @ w.t() + (3.0 if addend else 0.0)).float()
+    for tile in (0, pairs + 6):
+        D = torch.full((M, N), 9.5, device=DEV)                               
+        with LostCopy(ctx, tile):
+            ctx.gemm_fp8(A, B, D, N, Cin=Cin, ldc=N if addend else 0, stream=cur())
+            torch.cuda.synchronize()
+        tiles = lambda v: v.view(16, 256, 16, 256).transpose(1, 2).reshape(256, -1)  # noqa: E731
+        left = (tiles(D) == 9.5).all(1)
+        assert int(left.sum()) == len(range(tile, 256, pairs))
+        assert torch.equal(tiles(D)[~left], tiles(want)[~left])
+    assert torch.equal(run_gemm(ctx, A, B, torch.float32, Cin), want)
