@@ -127,7 +127,10 @@ struct decxb_ctx {
     int reserved_sms = 0;               /* SMs the next GEMM launches leave free (a transfer kernel runs beside them) */
     int inject_countdown = -1;          /* >= 0: that many pipeline CUDA calls from now, one reports a failure (tests) */
     std::atomic<int64_t> lost_copy{-1}; /* >= 0: the next launch that waits for copies leaves this row's or tile's out (tests) */
-    std::string last_error;
+    const uint64_t serial = ++serials;  /* an address may come back, this does not */
+    inline static std::atomic<uint64_t> serials{0};
+    std::mutex error_mtx;
+    std::string last_error;             /* of any thread; read by decxb_last_error */
     /* per-kernel event timing (decxb_profile_*) */
     bool profiling = false;
     std::mutex prof_mtx;

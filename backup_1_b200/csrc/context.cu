@@ -37,9 +37,20 @@ extern "C" const char* decxb_status_string(int status)
     }
 }
 
+/* The calling thread's own last failure, and the context it was on: threads that share a context each read the text of their
+ * own call, and no thread's text is written while another reads it. */
+static thread_local uint64_t own_error_ctx = 0;
+static thread_local std::string own_error, others_error;
+
 void decxb_set_error(decxb_ctx* ctx, const std::string& msg)
 {
-    if (ctx) ctx->last_error = msg;
+    if (!ctx) return;
+    {
+        std::lock_guard<std::mutex> lock(ctx->error_mtx);
+        ctx->last_error = msg;
+    }
+    own_error = msg;
+    own_error_ctx = ctx->serial;
 }
 
 int decxb_fail(decxb_ctx* ctx, int status, const std::string& msg)
@@ -50,7 +61,11 @@ int decxb_fail(decxb_ctx* ctx, int status, const std::string& msg)
 
 extern "C" const char* decxb_last_error(decxb_ctx* ctx)
 {
-    return ctx ? ctx->last_error.c_str() : "null context";
+    if (!ctx) return "null context";
+    if (own_error_ctx == ctx->serial) return own_error.c_str();
+    std::lock_guard<std::mutex> lock(ctx->error_mtx);
+    others_error = ctx->last_error;
+    return others_error.c_str();
 }
 
 int decxb_bind(decxb_ctx* ctx)

@@ -140,14 +140,14 @@ extern "C" int decxb_gemm_f32_noalloc(int device, int64_t M, int64_t N, int64_t 
     }
     if ((rc = decxb_launch_split_rows(ctx, A, M, K, lda, a_hi, a_lo, Kp, M, s)) ||
         (rc = decxb_launch_split_transpose(ctx, B, K, N, ldb, b_hi, b_lo, Kp, 0, s))) {
-        say(err, err_len, ctx->last_error.c_str()); return rc;
+        say(err, err_len, decxb_last_error(ctx)); return rc;
     }
     decxb_gemm_args g = {};
     g.M = M; g.N = N; g.K = K;
     g.a_hi = a_hi; g.a_lo = a_lo; g.lda = Kp;
     g.b_hi = b_hi; g.b_lo = b_lo; g.ldb = Kp; g.b_rows = N;
     g.C = C; g.ldc = ldc; g.D = D; g.ldd = ldd; g.tile = DECXB_TILE_AUTO;
-    if ((rc = decxb_launch_gemm_tn(ctx, g, s))) { say(err, err_len, ctx->last_error.c_str()); return rc; }
+    if ((rc = decxb_launch_gemm_tn(ctx, g, s))) { say(err, err_len, decxb_last_error(ctx)); return rc; }
     if (cudaStreamSynchronize(s) != cudaSuccess) {
         say(err, err_len, cudaGetErrorString(cudaGetLastError())); return DECXB_ERR_CUDA;
     }

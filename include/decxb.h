@@ -113,7 +113,8 @@ typedef struct decxb_ctx decxb_ctx;
 DECXB_API int decxb_init(int device, decxb_ctx** out);
 DECXB_API int decxb_destroy(decxb_ctx* ctx);
 DECXB_API const char* decxb_status_string(int status);
-/* Text of the last failure on this context (never NULL; valid until the next call). */
+/* Text of the calling thread's last failure on this context, or where it has had none (since it failed on another context) of any
+ * thread's last one (never NULL; valid until this thread's next call). */
 DECXB_API const char* decxb_last_error(decxb_ctx* ctx);
 DECXB_API int decxb_device(decxb_ctx* ctx);
 DECXB_API void* decxb_stream(decxb_ctx* ctx);

@@ -1091,3 +1091,39 @@ def test_product_of_many_tiles_leaves_tiles_that_did_not_come(ctx, b_rows, adden
         assert int(left.sum()) == len(range(tile, 256, pairs))
         assert torch.equal(tiles(D)[~left], tiles(want)[~left])
     assert torch.equal(run_gemm(ctx, A, B, torch.float32, Cin), want)
+
+
+# ---- two threads ---------------------------------------------------------------------------------------------------------
+@gpu
+def test_two_threads_are_refused_at_once_and_each_reads_its_own_text(ctx):
+    import threading
+
+    A, Q, x = b.Fp8Matrix.empty(4, 256), b.Fp8Matrix.empty(4, 256), torch.zeros((4, 256), device=DEV)
+    calls = [(lambda: ctx.gemm_fp8(A, A, x.data_ptr(), 3, d_type=b.F32, stream=cur()), "D: leading dimension smaller than the row length"),
+             (lambda: ctx.quantize_fp8(4, 256, x, 256, Q, rule=77, stream=cur()), "scale rule"),
+             (lambda: ctx.rmsnorm(4, 256, x, 256, x, -1.0, Y=x, ldy=256, stream=cur()), "eps must be a finite number >= 0")]
+    wrong, start = [], threading.Barrier(len(calls))
+
+    def work(call, text):
+        torch.cuda.set_device(0)
+        start.wait()
+        for _ in range(3000):
+            try:
+                call()
+                wrong.append("not refused")
+            except b.DecxbError as e:
+                if text not in str(e):
+                    wrong.append(str(e))
+    threads = [threading.Thread(target=work, args=c) for c in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong, wrong[:5]
+    with pytest.raises(b.DecxbError) as e:                  # this thread's own, though others failed later
+        ctx.quantize_fp8(4, 256, x, 256, None, stream=cur())
+    work_text = []
+    t = threading.Thread(target=lambda: work_text.append(ctx.L.decxb_last_error(ctx.h).decode()))
+    t.start()
+    t.join()
+    assert "nothing to write" in str(e.value) and "nothing to write" in work_text[0]       # a thread without a failure reads the last one
