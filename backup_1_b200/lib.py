@@ -196,6 +196,11 @@ _known_dtypes, _known_fp8 = {}, {}      # element type objects already looked up
 
 def _dtype(x, given):
     """F32 / F16 / BF16 of an array argument; `given` (needed for raw addresses) has to agree with a tensor's own."""
+    if given is None:
+        try:
+            return _known_dtypes[x.dtype]
+        except (AttributeError, KeyError):
+            pass
     dt = getattr(x, "dtype", None)
     own = _known_dtypes.get(dt)
     if own is None and dt is not None:
@@ -224,9 +229,22 @@ def _device_ptr(x):
     return _ptr(x)
 
 
+def _check_span(x, rows, ld, cols):
+    """Refuses a tensor that does not hold [rows][cols] elements of leading dimension `ld` from its address on, the columns of a
+    row contiguous.  Sizes that the entries refuse are left to them."""
+    shape, stride = tuple(x.shape), x.stride()
+    if shape and shape[-1] > 1 and stride[-1] != 1:
+        raise DecxbError(13, f"a tensor of shape {shape} and strides {stride}: the columns of a row must be contiguous")
+    have = 0 if 0 in shape else 1 + sum((n - 1) * s for n, s in zip(shape, stride))
+    elements = (rows - 1) * ld + cols
+    if have < elements and 0 < rows <= 0x7fffffff and cols > 0:
+        raise DecxbError(13, f"a tensor of shape {shape} and strides {stride} holds {have} elements, the call reaches {elements}")
+
+
 class Fp8Matrix:
     """An fp8 matrix with a scale for each block of block_rows x 128 codes (decxb_fp8_matrix): codes [rows][cols] with
-    row pitch `ld`, scale of element (r, c) at (r // block_rows) * scale_row_stride + (c // 128) * scale_block_stride."""
+    row pitch `ld`, scale of element (r, c) at (r // block_rows) * scale_row_stride + (c // 128) * scale_block_stride.
+    The sizes and strides given here are the caller's word; `of` takes them from the tensors."""
 
     def __init__(self, data, scales, rows, cols, ld, scale_row_stride, scale_block_stride, block_rows=1, type=FP8_E4M3):
         self.data, self.scales = data, scales          # kept alive with the descriptor
@@ -404,21 +422,40 @@ class Context:
         self._chk(self.L.decxb_gemm_release_b(self.h, pb, stream))
 
     # -- 8-bit linear layer -----------------------------------------------------------------
-    def _array(self, x, element):
-        """Address of an array argument of F32 / F16 / BF16 elements (None: of any type).  A tensor has to hold those and lie on
+    def _array(self, x, element, rows, ld, cols):
+        """Address of an array argument of F32 / F16 / BF16 elements.  A tensor has to hold [rows][cols] of those, `ld` apart, and lie on
         the context's device; a raw address is the caller's word."""
         if x is None:
             return None
         try:
-            if x.get_device() == self.device and (element is None or _known_dtypes[x.dtype] == element):
+            if (x.get_device() == self.device and _known_dtypes[x.dtype] == element and x.numel() >= (rows - 1) * ld + cols
+                    and x.is_contiguous()):
                 return x.data_ptr()
         except (AttributeError, KeyError):
             pass
-        if element is not None:
-            _dtype(x, element)
+        _dtype(x, element)
+        self._here(x)
+        if hasattr(x, "stride"):
+            _check_span(x, rows, ld, cols)
+        return _device_ptr(x)
+
+    def _bytes(self, x, nbytes):
+        """Address of a workspace argument; a tensor, of any type, has to hold `nbytes` bytes."""
+        if x is None:
+            return None
+        try:
+            if x.get_device() == self.device and x.numel() >= nbytes and x.is_contiguous():
+                return x.data_ptr()
+        except AttributeError:
+            pass
+        self._here(x)
+        if hasattr(x, "stride"):
+            _check_span(x, 1, 0, -(-nbytes // x.element_size()))
+        return _device_ptr(x)
+
+    def _here(self, x):
         if hasattr(x, "get_device") and x.get_device() != self.device:
             raise DecxbError(13, f"a tensor on {x.device} was passed to a context of cuda:{self.device}")
-        return _device_ptr(x)
 
     def _fp8(self, m):
         """Address of an fp8 matrix argument's descriptor."""
@@ -430,25 +467,28 @@ class Context:
 
     def _on(self, stream, some_tensor):
         """Handle of a `stream` argument.  Without one the work runs on the context's own stream, after what torch has queued."""
-        if stream is None:
-            if getattr(some_tensor, "is_cuda", False):
-                import torch
+        if stream is not None:
+            return _stream(stream)
+        if getattr(some_tensor, "is_cuda", False):
+            import torch
 
-                torch.cuda.current_stream(some_tensor.device).synchronize()
-            return None
-        return _stream(stream)
+            torch.cuda.current_stream(some_tensor.device).synchronize()
+        return None
 
     def gemm_fp8(self, A: Fp8Matrix, B: Fp8Matrix, D, ldd, Cin=None, ldc=0, d_type=None, stream=None):
         """D[A.rows][B.rows] = A B^T (+ Cin), both operands K-contiguous with their block scales (decxb_gemm_fp8)."""
         t, at = _dtype(D, d_type), self._array
-        rc = self.L.decxb_gemm_fp8(self.h, self._fp8(A), self._fp8(B), at(Cin, t), ldc, at(D, t), t, ldd, self._on(stream, A.data))
+        rc = self.L.decxb_gemm_fp8(self.h, self._fp8(A), self._fp8(B), at(Cin, t, A.rows, ldc, B.rows), ldc,
+                                   at(D, t, A.rows, ldd, B.rows), t, ldd, self._on(stream, A.data))
         if rc:
             self._chk(rc)
 
     def quantize_fp8(self, rows, cols, X, ldx, Q: Fp8Matrix = None, Qt: Fp8Matrix = None, rule=SCALE_AMAX, x_type=None, stream=None):
         """X [rows][cols] into Q and / or, transposed, into Qt (decxb_quantize_fp8)."""
         t = _dtype(X, x_type)
-        rc = self.L.decxb_quantize_fp8(self.h, t, rows, cols, self._array(X, t), ldx, rule, self._fp8(Q), self._fp8(Qt), self._on(stream, X))
+        agree = (Q is None or (Q.rows == rows and Q.cols == cols)) and (Qt is None or (Qt.rows == cols and Qt.cols == rows))
+        at = self._array(X, t, rows if agree else 0, ldx, cols)       # sizes that do not agree: the entry says which
+        rc = self.L.decxb_quantize_fp8(self.h, t, rows, cols, at, ldx, rule, self._fp8(Q), self._fp8(Qt), self._on(stream, X))
         if rc:
             self._chk(rc)
 
@@ -456,7 +496,8 @@ class Context:
                 rule=SCALE_AMAX, type=None, gamma_type=None, stream=None):
         """h = X (+ R), y = h / rms(h) * gamma into H, Y and, quantised, Q, whichever are given (decxb_rmsnorm)."""
         t, tg, at = _dtype(X, type), _dtype(gamma, gamma_type), self._array
-        rc = self.L.decxb_rmsnorm(self.h, t, rows, cols, at(X, t), ldx, at(R, t), ldr, at(gamma, tg), tg, eps, at(H, t), ldh, at(Y, t), ldy,
+        rc = self.L.decxb_rmsnorm(self.h, t, rows, cols, at(X, t, rows, ldx, cols), ldx, at(R, t, rows, ldr, cols), ldr,
+                                  at(gamma, tg, 1, 0, cols), tg, eps, at(H, t, rows, ldh, cols), ldh, at(Y, t, rows, ldy, cols), ldy,
                                   rule, self._fp8(Q), self._on(stream, X))
         if rc:
             self._chk(rc)
@@ -470,8 +511,10 @@ class Context:
                          workspace=None, workspace_bytes=0, type=None, gamma_type=None, stream=None):
         """Gradients of rmsnorm's y: dX (with dR added) and dgamma, fp32 (decxb_rmsnorm_backward)."""
         t, tg, at = _dtype(H, type), _dtype(gamma, gamma_type), self._array
-        rc = self.L.decxb_rmsnorm_backward(self.h, t, rows, cols, at(dY, t), lddy, at(H, t), ldh, at(gamma, tg), tg, eps, at(dR, t), lddr,
-                                           at(dX, t), lddx, at(dgamma, F32), at(workspace, None), workspace_bytes, self._on(stream, gamma))
+        rc = self.L.decxb_rmsnorm_backward(self.h, t, rows, cols, at(dY, t, rows, lddy, cols), lddy, at(H, t, rows, ldh, cols), ldh,
+                                           at(gamma, tg, 1, 0, cols), tg, eps, at(dR, t, rows, lddr, cols), lddr,
+                                           at(dX, t, rows, lddx, cols), lddx, at(dgamma, F32, 1, 0, cols),
+                                           self._bytes(workspace, workspace_bytes), workspace_bytes, self._on(stream, gamma))
         if rc:
             self._chk(rc)
 

@@ -1127,3 +1127,62 @@ def test_two_threads_are_refused_at_once_and_each_reads_its_own_text(ctx):
     t.start()
     t.join()
     assert "nothing to write" in str(e.value) and "nothing to write" in work_text[0]       # a thread without a failure reads the last one
+
+
+# ---- tensors that do not hold what a call reaches -----------------------------------------------------------------------
+class Entries:
+    """The library, as far as a call that has been let through goes: nothing runs."""
+
+    def __init__(self):
+        self.calls = 0
+
+    def __getattr__(self, name):
+        def entry(*args):
+            self.calls += 1
+            return 0
+        return entry
+
+
+def host_context():
+    """A context whose device is the host's memory (-1, as its tensors say) and whose entries do nothing."""
+    c = b.Context.__new__(b.Context)
+    c.L, c.h, c.device = Entries(), None, -1
+    return c
+
+
+def test_tensors_that_are_too_small_or_not_rows_are_refused():
+    c, e = host_context(), torch.empty
+    bf = dict(dtype=torch.bfloat16)
+    A, W, Q, T = (b.Fp8Matrix.empty(r, k, br, device="cpu") for r, k, br in [(4, 256, 1), (8, 256, 128), (4, 256, 1), (256, 4, 1)])
+    x, gamma, wide = e(4, 256, **bf), e(256), e(4, 300, **bf)[:, :256]
+    ok = [lambda: c.gemm_fp8(A, W, e(4, 8), 8), lambda: c.gemm_fp8(A, W, e(3 * 11 + 8), 11, Cin=e(4, 8), ldc=8),
+          lambda: c.gemm_fp8(A, W, e(4, 20)[:, :8], 20), lambda: c.gemm_fp8(A, W, 4096, 8, d_type=b.F16),
+          lambda: c.quantize_fp8(4, 256, x, 256, Q, T), lambda: c.quantize_fp8(4, 256, wide, 300, Q), lambda: c.quantize_fp8(4, 256, e(2, 2, 256), 256, Q),
+          lambda: c.quantize_fp8(1, 256, e(256), 256, b.Fp8Matrix.empty(1, 256, device="cpu")),
+          lambda: c.quantize_fp8(0, 256, e(0, 256), 256, b.Fp8Matrix.empty(0, 256, device="cpu")),
+          lambda: c.rmsnorm(4, 256, wide, 300, gamma, 1e-6, R=x, ldr=256, H=x, ldh=256, Y=wide, ldy=300, Q=Q),
+          lambda: c.rmsnorm_backward(4, 256, x, 256, wide, 300, gamma, 1e-6, x, 256, gamma, dR=x, lddr=256, workspace=e(300), workspace_bytes=1200),
+          lambda: c.rmsnorm_backward(0, 256, x, 256, x, 256, gamma, 1e-6, x, 256, gamma)]
+    for call in ok:
+        call()
+    assert c.L.calls == len(ok)
+    g2 = e(512)[::2]
+    bad = [lambda: c.gemm_fp8(A, W, e(4, 7), 8), lambda: c.gemm_fp8(A, W, e(3, 8), 8), lambda: c.gemm_fp8(A, W, e(3 * 11 + 7), 11),
+           lambda: c.gemm_fp8(A, W, e(8, 4).t(), 8), lambda: c.gemm_fp8(A, W, e(4, 8), 8, Cin=e(8).expand(4, 8), ldc=8),
+           lambda: c.gemm_fp8(A, W, e(4, 8), 8, Cin=e(3, 8), ldc=8),
+           lambda: c.quantize_fp8(4, 256, e(3, 256), 256, Q), lambda: c.quantize_fp8(4, 256, e(256, 4).t(), 256, Q), lambda: c.quantize_fp8(4, 256, wide, 301, Q),
+           lambda: c.quantize_fp8(4, 256, e(1, 256).expand(4, 256), 256, Q), lambda: c.quantize_fp8(4, 256, x[3:], 256, None, T),
+           lambda: c.rmsnorm(4, 256, x[1:], 256, gamma, 1e-6, Q=Q), lambda: c.rmsnorm(4, 256, x, 256, gamma[1:], 1e-6, Q=Q),
+           lambda: c.rmsnorm(4, 256, x, 256, g2, 1e-6, Q=Q), lambda: c.rmsnorm(4, 256, x, 256, gamma, 1e-6, R=x, ldr=257, Q=Q),
+           lambda: c.rmsnorm(4, 256, x, 256, gamma, 1e-6, H=x[:3], ldh=256), lambda: c.rmsnorm(4, 256, x, 256, gamma, 1e-6, Y=x[:3], ldy=256),
+           lambda: c.rmsnorm_backward(4, 256, x[1:], 256, x, 256, gamma, 1e-6, x, 256), lambda: c.rmsnorm_backward(4, 256, x, 256, x[1:], 256, gamma, 1e-6, x, 256),
+           lambda: c.rmsnorm_backward(4, 256, x, 256, x, 256, gamma[1:], 1e-6, x, 256), lambda: c.rmsnorm_backward(4, 256, x, 256, x, 256, gamma, 1e-6, x[1:], 256),
+           lambda: c.rmsnorm_backward(4, 256, x, 256, x, 256, gamma, 1e-6, x, 256, e(255)), lambda: c.rmsnorm_backward(4, 256, x, 256, x, 256, gamma, 1e-6, x, 256, g2),
+           lambda: c.rmsnorm_backward(0, 256, x, 256, x, 256, gamma, 1e-6, x, 256, e(255)),
+           lambda: c.rmsnorm_backward(4, 256, x, 256, x, 256, gamma, 1e-6, x, 256, dR=x[1:], lddr=256),
+           lambda: c.rmsnorm_backward(4, 256, x, 256, x, 256, gamma, 1e-6, x, 256, gamma, workspace=e(299), workspace_bytes=1200)]
+    for i, call in enumerate(bad):
+        with pytest.raises(b.DecxbError) as err:
+            call()
+        assert err.value.status == 13, i
+    assert c.L.calls == len(ok)
