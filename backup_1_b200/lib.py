@@ -215,11 +215,11 @@ def _dtype(x, given):
 
 
 def _stream(stream):
-    """Raw handle of a `stream` argument: None (the context's own stream), an address, or a torch stream.  Torch's default
-    stream has the address 0, which the C ABI reads as the context's own; it is passed by its explicit handle, 1."""
-    if stream is None or isinstance(stream, int):
-        return stream
-    return stream.cuda_stream or 1
+    """Raw handle of a `stream` argument: None (the context's own stream), a handle, or a torch stream.  CUDA's default stream,
+    which is torch's too, has the handle 0, which the C ABI reads as the context's own; it is passed by its explicit handle, 1."""
+    if stream is None:
+        return None
+    return (stream if isinstance(stream, int) else stream.cuda_stream) or 1
 
 
 def _device_ptr(x):
@@ -465,21 +465,26 @@ class Context:
             raise DecxbError(13, f"an fp8 matrix on device {m.device} was passed to a context of cuda:{self.device}")
         return m.addr
 
-    def _on(self, stream, some_tensor):
-        """Handle of a `stream` argument.  Without one the work runs on the context's own stream, after what torch has queued."""
+    def _on(self, stream, *arrays):
+        """Handle of a `stream` argument.  Without one the work runs on the context's own stream, after what torch has queued: asked
+        if any of `arrays` is torch's."""
         if stream is not None:
             return _stream(stream)
-        if getattr(some_tensor, "is_cuda", False):
-            import torch
+        for x in arrays:
+            if isinstance(x, Fp8Matrix):
+                x = x.data
+            if getattr(x, "is_cuda", False):
+                import torch
 
-            torch.cuda.current_stream(some_tensor.device).synchronize()
+                torch.cuda.current_stream(x.device).synchronize()
+                break
         return None
 
     def gemm_fp8(self, A: Fp8Matrix, B: Fp8Matrix, D, ldd, Cin=None, ldc=0, d_type=None, stream=None):
         """D[A.rows][B.rows] = A B^T (+ Cin), both operands K-contiguous with their block scales (decxb_gemm_fp8)."""
         t, at = _dtype(D, d_type), self._array
         rc = self.L.decxb_gemm_fp8(self.h, self._fp8(A), self._fp8(B), at(Cin, t, A.rows, ldc, B.rows), ldc,
-                                   at(D, t, A.rows, ldd, B.rows), t, ldd, self._on(stream, A.data))
+                                   at(D, t, A.rows, ldd, B.rows), t, ldd, self._on(stream, A, B, D, Cin))
         if rc:
             self._chk(rc)
 
@@ -488,7 +493,7 @@ class Context:
         t = _dtype(X, x_type)
         agree = (Q is None or (Q.rows == rows and Q.cols == cols)) and (Qt is None or (Qt.rows == cols and Qt.cols == rows))
         at = self._array(X, t, rows if agree else 0, ldx, cols)       # sizes that do not agree: the entry says which
-        rc = self.L.decxb_quantize_fp8(self.h, t, rows, cols, at, ldx, rule, self._fp8(Q), self._fp8(Qt), self._on(stream, X))
+        rc = self.L.decxb_quantize_fp8(self.h, t, rows, cols, at, ldx, rule, self._fp8(Q), self._fp8(Qt), self._on(stream, X, Q, Qt))
         if rc:
             self._chk(rc)
 
@@ -498,7 +503,7 @@ class Context:
         t, tg, at = _dtype(X, type), _dtype(gamma, gamma_type), self._array
         rc = self.L.decxb_rmsnorm(self.h, t, rows, cols, at(X, t, rows, ldx, cols), ldx, at(R, t, rows, ldr, cols), ldr,
                                   at(gamma, tg, 1, 0, cols), tg, eps, at(H, t, rows, ldh, cols), ldh, at(Y, t, rows, ldy, cols), ldy,
-                                  rule, self._fp8(Q), self._on(stream, X))
+                                  rule, self._fp8(Q), self._on(stream, X, R, gamma, H, Y, Q))
         if rc:
             self._chk(rc)
 
@@ -514,7 +519,7 @@ class Context:
         rc = self.L.decxb_rmsnorm_backward(self.h, t, rows, cols, at(dY, t, rows, lddy, cols), lddy, at(H, t, rows, ldh, cols), ldh,
                                            at(gamma, tg, 1, 0, cols), tg, eps, at(dR, t, rows, lddr, cols), lddr,
                                            at(dX, t, rows, lddx, cols), lddx, at(dgamma, F32, 1, 0, cols),
-                                           self._bytes(workspace, workspace_bytes), workspace_bytes, self._on(stream, gamma))
+                                           self._bytes(workspace, workspace_bytes), workspace_bytes, self._on(stream, dY, H, gamma, dR, dX, dgamma, workspace))
         if rc:
             self._chk(rc)
 

@@ -1186,3 +1186,68 @@ def test_tensors_that_are_too_small_or_not_rows_are_refused():
             call()
         assert err.value.status == 13, i
     assert c.L.calls == len(ok)
+
+
+def test_the_default_streams_handle_is_not_the_contexts_own_stream():
+    assert blib._stream(0) == 1 and blib._stream(2) == 2
+
+
+def test_calls_without_a_stream_wait_for_torch_whichever_argument_is_torchs(monkeypatch):
+    waits = []
+
+    class OnDevice:
+        """As much of a CUDA tensor as a call looks at."""
+        is_cuda, device, dtype = True, "cuda:0", torch.float32
+
+        def get_device(self):
+            return -1
+
+        def numel(self):
+            return 1 << 20
+
+        def is_contiguous(self):
+            return True
+
+        def data_ptr(self):
+            return 4096
+
+    class Stream:
+        def synchronize(self):
+            waits.append(1)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream())
+    c, t, p = host_context(), OnDevice(), 4096
+    raw = b.Fp8Matrix(p, p, 4, 256, 256, 1, 4)
+    raw_t, mixed = b.Fp8Matrix(p, p, 256, 4, 16, 1, 256), b.Fp8Matrix(p, p, 4, 256, 256, 1, 4)
+    mixed.data = t
+    f = dict(x_type=b.F32)
+    calls = [lambda **s: c.gemm_fp8(raw, raw, t, 4, **s), lambda **s: c.gemm_fp8(raw, mixed, p, 4, d_type=b.F32, **s),
+             lambda **s: c.gemm_fp8(raw, raw, p, 4, Cin=t, ldc=4, d_type=b.F32, **s),
+             lambda **s: c.quantize_fp8(4, 256, p, 256, mixed, **f, **s), lambda **s: c.quantize_fp8(4, 256, t, 256, raw, raw_t, **s),
+             lambda **s: c.rmsnorm(4, 256, p, 256, p, 1e-6, Y=t, ldy=256, type=b.F32, gamma_type=b.F32, **s),
+             lambda **s: c.rmsnorm(4, 256, p, 256, t, 1e-6, Y=p, ldy=256, type=b.F32, **s),
+             lambda **s: c.rmsnorm_backward(4, 256, t, 256, p, 256, p, 1e-6, p, 256, type=b.F32, gamma_type=b.F32, **s),
+             lambda **s: c.rmsnorm_backward(4, 256, p, 256, p, 256, p, 1e-6, p, 256, t, type=b.F32, gamma_type=b.F32, **s)]
+    for i, call in enumerate(calls):
+        call()
+        assert len(waits) == i + 1, i
+    for call in calls:
+        call(stream=7)
+    c.gemm_fp8(raw, raw, p, 4, d_type=b.F32)               # nothing of torch's
+    assert len(waits) == len(calls)
+
+
+@gpu
+def test_a_call_on_the_default_streams_handle_follows_what_is_queued_there(ctx):
+    """The input is still being written when the call is made, and torch reads the result without waiting."""
+    rows, cols = 4096, 4096
+    x = torch.empty(rows, cols, device=DEV)
+    gamma, Y = torch.ones(cols, device=DEV), torch.zeros(rows, cols, device=DEV)
+    big = torch.randn(8192, 8192, device=DEV)
+    with torch.cuda.stream(torch.cuda.default_stream()):
+        for _ in range(8):
+            big = big @ big * 1e-2                          # some milliseconds
+        x.fill_(2.0)
+        ctx.rmsnorm(rows, cols, x, cols, gamma, 0.0, Y=Y, ldy=cols, stream=torch.cuda.current_stream().cuda_stream)
+        got = Y.clone()
+    torch.cuda.synchronize()
+    assert bool((got - 1).abs().max() <= 8 * U)
