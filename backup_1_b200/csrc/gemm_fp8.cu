@@ -659,7 +659,7 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
  * ------------------------------------------------------------------------------------ */
 template <int NT>
 struct SplitCfg {
-    static constexpr int CTAS_PER_SM = NT == 128 ? 1 : 2;      /* at most, when the launch asks for half of the shared memory */
+    static constexpr int CTAS_PER_SM = NT == 128 ? 1 : 2;      /* at most, when the launch asks for half of the shared memory (no clusters then) */
     static constexpr int CW = NT / 2;                          /* columns per epilogue warp */
     static constexpr int W_BYTES = BM_CTA * BK;
     static constexpr int STAGE_BYTES = W_BYTES + NT * BK;
@@ -1013,10 +1013,12 @@ const Resident& resident(decxb_ctx* ctx)
  *  - The largest power of two of shares of which one wave of clusters holds all (2048 columns, K = 4096, one token: 2, 4, 8
  *    shares 6.6, 4.7, 8.2 us, eight being two waves), but no share below four k-blocks (1 x 4096 x 1024: two shares
  *    3.9, four 4.3, eight 5.2 us).
- *  - Up to 64 tokens, where that leaves a fifth of the SMs empty, twice the shares with two CTAs to an SM (1 x 12000 x 4096:
- *    11.4 and 10.3 us; 1 x 6000 x 4096: 7.3 and 6.9), though not eight (33 x 2048 x 4096, four and eight: 6.4 and 7.1).
- *    Two CTAs to an SM as well where there are more tiles than SMs (64 x 32768 x 4096: 32.3 and 26.4). Otherwise one CTA
- *    with all of the shared memory has the longer queue of loads (48 x 4096 x 8192: 10.3 and 14.6). */
+ *  - Up to 64 tokens, two CTAs to an SM where there are more tiles than SMs (64 x 32768 x 4096: 32.3 and 26.4). Otherwise one CTA
+ *    with all of the shared memory has the longer queue of loads (48 x 4096 x 8192: 10.3 and 14.6).
+ *  - Never a cluster of CTAs that leave room on their SMs: tensor memory is taken in the order in which blocks come, without
+ *    a limit to the wait, and a CTA that holds some while it waits for its peer, next to a block of another kernel that does the same
+ *    the other way round, would wait for good.  (Twice the shares with two CTAs to an SM, where a fifth of the SMs are
+ *    empty: 1 x 6000 x 4096 6.97 -> 6.56 us, 40 x 5000 x 4096 9.4 -> 10.1.) */
 struct Cut { int splits, per_sm; double us; };
 
 template <int NT>
@@ -1031,10 +1033,7 @@ int plan_split(decxb_ctx* ctx, int64_t M, int64_t N, int num_kb, Cut* out)
     const int fit = r.clusters[i] > 0 ? r.clusters[i] : 1;
     const int64_t waves = decxb_ceil_div(tiles, fit);
     c.us = 5.0 + (waves > 1 ? 0.50 : 0.36) * (double)waves * (double)decxb_ceil_div(num_kb, c.splits);
-    if (SplitCfg<NT>::CTAS_PER_SM == 2) {
-        if (tiles > fit) c.per_sm = 2;
-        else if (i < 2 && tiles * c.splits * 5 < (int64_t)ctx->sm_count * 4 && num_kb >= (8 << i)) { c.splits *= 2; c.per_sm = 2; }
-    }
+    if (SplitCfg<NT>::CTAS_PER_SM == 2 && tiles > fit) c.per_sm = 2;
     *out = c;
     return DECXB_OK;
 }

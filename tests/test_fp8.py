@@ -1251,3 +1251,32 @@ def test_a_call_on_the_default_streams_handle_follows_what_is_queued_there(ctx):
         got = Y.clone()
     torch.cuda.synchronize()
     assert bool((got - 1).abs().max() <= 8 * U)
+
+
+@gpu
+def test_products_of_every_form_side_by_side(ctx):
+    """Four streams with products of one token to many, cut over clusters, two blocks to an SM and pairs, all at once: exact, and all end."""
+    g = gen(35)
+    shapes = [(1, 4096, 2048), (1, 6000, 4096), (20, 12000, 1024), (64, 20000, 512), (40, 5000, 4096), (100, 512, 2048), (2048, 1280, 384), (1, 20000, 640)]
+    made = []
+    for M, N, K in shapes:
+        A, a = int_matrix(g, M, K, b.FP8_E4M3, 1)
+        B, w = int_matrix(g, N, K, b.FP8_E4M3, 128)
+        made.append((A, B, torch.empty((M, N), device=DEV), (a @ w.t()).float()))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    for turn in range(12):
+        for i, s in enumerate(streams):
+            for j in range(len(made)):
+                A, B, D, _ = made[(j + turn + 2 * i) % len(made)]
+                if j % 4 == i:
+                    ctx.gemm_fp8(A, B, D, D.shape[1], stream=s)
+        torch.cuda.synchronize()
+    ctx.synchronize()
+    for A, B, D, want in made:
+        for s in streams:
+            D.fill_(-1.0)
+            torch.cuda.synchronize()
+            ctx.gemm_fp8(A, B, D, D.shape[1], stream=s)
+            torch.cuda.synchronize()
+            assert torch.equal(D, want)
