@@ -26,8 +26,12 @@ namespace {
 
 constexpr int PROBE_THREADS = 128;
 constexpr int TILE_BYTES = 128 * 32 * 4;                 /* 16 KiB: 128 rows of one 128-byte k-block (an A tile) */
-/* a_hi, a_lo (128 rows each), b_hi, b_lo (BN rows each), alignment slack, barrier + TMEM slot */
-constexpr int probe_smem(int bn) { return 2 * TILE_BYTES + 2 * bn * 128 + 1024 + 64; }
+/* a_hi, a_lo (128 rows each), b_hi, b_lo (BN rows each), alignment slack, barrier + TMEM slot; and the rest of the SM's, so that no other
+ * block that holds tensor memory shares the SM: a pair that has its columns on one SM and waits for those on the other, without a limit,
+ * could wait for a pair that does the same the other way round */
+constexpr int PROBE_SMEM = 232448;
+constexpr int probe_needs(int bn) { return 2 * TILE_BYTES + 2 * bn * 128 + 1024 + 64; }
+static_assert(probe_needs(256) <= PROBE_SMEM, "shared memory");
 
 __device__ __forceinline__ uint32_t mix32(uint32_t h)
 {
@@ -114,12 +118,12 @@ template <int PATTERN, int CTAS, int BN>
 int launch_probe(decxb_ctx* ctx, int iters, cudaStream_t s)
 {
     auto kernel = decxb_tensor_probe_kernel<PATTERN, CTAS, BN>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, probe_smem(BN));
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PROBE_SMEM);
     if (e != cudaSuccess) return decxb_fail(ctx, DECXB_ERR_CUDA, std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(ctx->sm_count / CTAS * CTAS), 1, 1);
     cfg.blockDim = dim3(PROBE_THREADS, 1, 1);
-    cfg.dynamicSmemBytes = probe_smem(BN);
+    cfg.dynamicSmemBytes = PROBE_SMEM;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;

@@ -1280,3 +1280,34 @@ def test_products_of_every_form_side_by_side(ctx):
             ctx.gemm_fp8(A, B, D, D.shape[1], stream=s)
             torch.cuda.synchronize()
             assert torch.equal(D, want)
+
+
+@gpu
+def test_tensor_probes_of_two_contexts_beside_products(ctx):
+    """Two threads probe the tensor cores, each on its own context, while products run on two more streams: all end, the products are exact."""
+    import threading
+
+    other, g = b.Context(0), gen(36)
+    made = []
+    for M, N, K in [(1, 6000, 4096), (64, 20000, 512), (2048, 1280, 384)]:
+        A, a = int_matrix(g, M, K, b.FP8_E4M3, 1)
+        B, w = int_matrix(g, N, K, b.FP8_E4M3, 128)
+        made.append((A, B, torch.empty((M, N), device=DEV), (a @ w.t()).float()))
+    torch.cuda.synchronize()
+    rates = []
+    threads = [threading.Thread(target=lambda c=c, p=p: rates.append(c.probe_tensor_peak(p, 20.0)["tensor_tflops"])) for c, p in ((ctx, 1), (other, 3))]
+    for t in threads:
+        t.start()
+    streams = [torch.cuda.Stream() for _ in made]
+    for _ in range(100):
+        for (A, B, D, _), s in zip(made, streams):
+            ctx.gemm_fp8(A, B, D, D.shape[1], stream=s)
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    ctx.synchronize()
+    other.synchronize()
+    other.close()
+    assert len(rates) == 2 and min(rates) > 0
+    for _, _, D, want in made:
+        assert torch.equal(D, want)
