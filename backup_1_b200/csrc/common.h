@@ -23,6 +23,7 @@ struct decxb_dev_status {
     int where;       /* role/barrier id that gave up                       */
     int block;       /* blockIdx.x of the reporter                         */
     int detail;      /* stage / tile index                                 */
+    unsigned int launch;   /* launch of the 8-bit layer in which a wait gave up last (its `Waits::launch`); 0: none */
 };
 
 /* Per-device tables (kernel attributes set once per device) are sized by this; decxb_init
@@ -126,6 +127,7 @@ struct decxb_ctx {
     int tile_group = 8;                 /* tile-rows per group of the GEMM kernel's tile order (decxb_set_tile_group) */
     int reserved_sms = 0;               /* SMs the next GEMM launches leave free (a transfer kernel runs beside them) */
     int inject_countdown = -1;          /* >= 0: that many pipeline CUDA calls from now, one reports a failure (tests) */
+    std::atomic<uint64_t> wait_launches{0};     /* launches of the 8-bit layer with waits */
     std::atomic<int64_t> lost_copy{-1}; /* >= 0: the next launch that waits for copies leaves this row's or tile's out (tests) */
     const uint64_t serial = ++serials;  /* an address may come back, this does not */
     inline static std::atomic<uint64_t> serials{0};

@@ -193,6 +193,25 @@ __device__ __forceinline__ void store_codes8(uint8_t* p, int n, bool vec, uint2 
     }
 }
 
+/* ------------------------------------------------------------------ waits ------------ */
+/* What a launch's waits go by.  A wait that lasts longer than the limit gives up, and the launch's other waits with it; those of other
+ * launches do not, since what they wait for may well come. */
+struct Waits {
+    decxb_dev_status* status;
+    long long limit_ns;
+    uint32_t launch;                  /* this launch's number, not 0                         */
+    int64_t lost;                     /* row or tile whose copies are left out (tests; -1: none) */
+};
+__device__ __forceinline__ bool gave_up(const Waits& w) { return *reinterpret_cast<volatile uint32_t*>(&w.status->launch) == w.launch; }
+__device__ __forceinline__ void give_up(const Waits& w, int where, int detail)
+{
+    if (atomicCAS(&w.status->code, 0, DECXB_DEVERR_WAIT_EXPIRED) == 0) {
+        w.status->where = where; w.status->block = (int)blockIdx.x; w.status->detail = detail;
+    }
+    *reinterpret_cast<volatile uint32_t*>(&w.status->launch) = w.launch;
+    __threadfence_system();
+}
+
 /* ------------------------------------------------------------------ host side -------- */
 /* Makes the context's device current for one entry and puts the caller's back. */
 struct DeviceScope {
@@ -257,9 +276,12 @@ inline int refuse_capture(decxb_ctx* ctx, cudaStream_t s, const char* what)
     return DECXB_OK;
 }
 
-/* The row (of a norm) or result tile (of a product) whose copies the next launch that waits for copies leaves out, once
- * (decxb_inject_lost_copy); -1: none. */
-inline int64_t lost_copy(decxb_ctx* ctx) { return ctx->lost_copy.load(std::memory_order_relaxed) < 0 ? -1 : ctx->lost_copy.exchange(-1); }
+/* Of the next launch; it alone leaves out the copies that decxb_inject_lost_copy names. */
+inline Waits waits_of(decxb_ctx* ctx)
+{
+    const int64_t lost = ctx->lost_copy.load(std::memory_order_relaxed) < 0 ? -1 : ctx->lost_copy.exchange(-1);
+    return {ctx->d_status, ctx->wait_limit_ns, (uint32_t)(ctx->wait_launches++ % 0xffffffffu) + 1u, lost};
+}
 
 }  // namespace fp8
 #endif

@@ -47,21 +47,17 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                  :: "r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
 
-/* Wait for a stage's copies.  False where they did not come within the limit, which the status word then says, or where
- * another wait had given up before. */
-__device__ __forceinline__ bool wait_copy(uint32_t bar, uint32_t parity, long long limit_ns, decxb_dev_status* status)
+/* Wait for a stage's copies.  False where they did not come within the limit, or another wait of the launch had given up before. */
+__device__ __forceinline__ bool wait_copy(uint32_t bar, uint32_t parity, const Waits& w)
 {
     unsigned long long t0 = 0;
     for (uint32_t spins = 1; !tcptx::mbar_try_wait(bar, parity); ++spins) {
         if (spins & 1023u) continue;
-        if (*reinterpret_cast<volatile int*>(&status->code) != 0) return false;
+        if (gave_up(w)) return false;
         const unsigned long long t = tcptx::globaltimer_ns();
         if (t0 == 0) t0 = t;
-        if ((long long)(t - t0) > limit_ns) {
-            if (atomicCAS(&status->code, 0, DECXB_DEVERR_WAIT_EXPIRED) == 0) {
-                status->where = 3000; status->block = (int)blockIdx.x; status->detail = 0;
-                __threadfence_system();
-            }
+        if ((long long)(t - t0) > w.limit_ns) {
+            give_up(w, 3000, 0);
             return false;
         }
     }
@@ -180,11 +176,10 @@ decxb_rmsnorm_kernel(const NormArgs a)
  * instructions: reads and writes share the memory best when neither runs far ahead. */
 template <typename T>
 __global__ void __launch_bounds__(512, 3)
-decxb_rmsnorm_rows_kernel(const NormArgs a, const int stages, const long long wait_limit_ns, decxb_dev_status* status, const int64_t lost_row)
+decxb_rmsnorm_rows_kernel(const NormArgs a, const int stages, const Waits waits)
 {
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ float part[2][16];
-    __shared__ int lost[2];                    /* a thread gave its wait up; alternates with `part` */
+    __shared__ float part[2][17];              /* [16]: not 0 where a thread gave its wait up */
     __shared__ __align__(8) uint64_t bars[8];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nwarps = blockDim.x >> 5, cols = (int)a.cols;
     const int arrays = a.r ? 2 : 1;
@@ -193,12 +188,12 @@ decxb_rmsnorm_rows_kernel(const NormArgs a, const int stages, const long long wa
     auto fetch = [&](int64_t row, int st) {
         const uint32_t bar = tcptx::smem_u32(&bars[st]), at = tcptx::smem_u32(smem) + (uint32_t)(st * arrays) * row_bytes;
         tcptx::mbar_arrive_expect_tx(bar, row_bytes * arrays);
-        if (row == lost_row) return;
+        if (row == waits.lost) return;
         bulk_load(at, static_cast<const T*>(a.x) + row * a.ldx, row_bytes, bar);
         if (a.r) bulk_load(at + row_bytes, static_cast<const T*>(a.r) + row * a.ldr, row_bytes, bar);
     };
     if (tid == 0) {
-        lost[0] = lost[1] = 0;
+        part[0][16] = part[1][16] = 0.0f;
         for (int st = 0; st < stages; ++st) tcptx::mbar_init(tcptx::smem_u32(&bars[st]), 1);
         tcptx::fence_barrier_init();
     }
@@ -212,7 +207,7 @@ decxb_rmsnorm_rows_kernel(const NormArgs a, const int stages, const long long wa
     const float of_cols = 1.0f / (float)cols;
     int st = 0, turn = 0; uint32_t phase = 0;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
-        if (!wait_copy(tcptx::smem_u32(&bars[st]), phase, wait_limit_ns, status)) lost[turn] = 1;
+        if (!wait_copy(tcptx::smem_u32(&bars[st]), phase, waits)) part[turn][16] = 1.0f;
         const T* in = reinterpret_cast<const T*>(smem + (size_t)(st * arrays) * row_bytes);
         float v[8], sum = 0.0f;
         load8(in + first, n, true, v);
@@ -227,7 +222,7 @@ decxb_rmsnorm_rows_kernel(const NormArgs a, const int stages, const long long wa
         sum = warp_sum(sum);
         if (lane == 0) part[turn][warp] = sum;
         __syncthreads();                       /* every thread has its values: the stage can be filled again */
-        if (lost[turn]) {                      /* the row did not come: it and those behind it stay unwritten */
+        if (part[turn][16] != 0.0f) {          /* the row did not come: it and those behind it stay unwritten */
             if (tid == 0) drain_copies(bars, stages, st, phase, row, a.rows);
             return;
         }
@@ -317,7 +312,7 @@ int launch_norm_many(decxb_ctx* ctx, const NormArgs& a, cudaStream_t s)
     std::call_once(once[ctx->device], [&] { err[ctx->device] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 32 * 1024); });
     if (err[ctx->device] != cudaSuccess) return decxb_fail(ctx, DECXB_ERR_CUDA, std::string("norm kernel attributes: ") + cudaGetErrorString(err[ctx->device]));
     return launch_after(ctx, kernel, (unsigned)(2 * ctx->sm_count), threads_for(decxb_ceil_div(a.cols, 8), 1, 512), smem, s, a, stages,
-                        ctx->wait_limit_ns, ctx->d_status, lost_copy(ctx));
+                        waits_of(ctx));
 }
 
 /* One vector a thread as far as 1024 threads reach (8192 x 4096 bf16 with one, two, four: 64, 69, 74 us): a block's loads,
@@ -410,11 +405,10 @@ decxb_rmsnorm_backward_kernel(const NormBwdArgs a)
  * 122 us with loads into registers). */
 template <typename T, int VPT>
 __global__ void __launch_bounds__(512, VPT == 1 ? 2 : 1)
-decxb_rmsnorm_backward_rows_kernel(const NormBwdArgs a, const int stages, const long long wait_limit_ns, decxb_dev_status* status, const int64_t lost_row)
+decxb_rmsnorm_backward_rows_kernel(const NormBwdArgs a, const int stages, const Waits waits)
 {
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ float2 buf[2][16];
-    __shared__ int lost[2];                    /* a thread gave its wait up; alternates with `buf` */
+    __shared__ float2 buf[2][17];              /* [16]: not 0 where a thread gave its wait up */
     __shared__ __align__(8) uint64_t bars[8];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nwarps = blockDim.x >> 5, cols = (int)a.cols;
     const int arrays = a.dr ? 3 : 2;
@@ -423,13 +417,13 @@ decxb_rmsnorm_backward_rows_kernel(const NormBwdArgs a, const int stages, const 
     auto fetch = [&](int64_t row, int st) {
         const uint32_t bar = tcptx::smem_u32(&bars[st]), at = tcptx::smem_u32(smem) + (uint32_t)(st * arrays) * row_bytes;
         tcptx::mbar_arrive_expect_tx(bar, row_bytes * arrays);
-        if (row == lost_row) return;
+        if (row == waits.lost) return;
         bulk_load(at, static_cast<const T*>(a.dy) + row * a.lddy, row_bytes, bar);
         bulk_load(at + row_bytes, static_cast<const T*>(a.h) + row * a.ldh, row_bytes, bar);
         if (a.dr) bulk_load(at + 2 * row_bytes, static_cast<const T*>(a.dr) + row * a.lddr, row_bytes, bar);
     };
     if (tid == 0) {
-        lost[0] = lost[1] = 0;
+        buf[0][16].x = buf[1][16].x = 0.0f;
         for (int st = 0; st < stages; ++st) tcptx::mbar_init(tcptx::smem_u32(&bars[st]), 1);
         tcptx::fence_barrier_init();
     }
@@ -452,7 +446,7 @@ decxb_rmsnorm_backward_rows_kernel(const NormBwdArgs a, const int stages, const 
     }
     int st = 0, turn = 0; uint32_t phase = 0;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
-        if (!wait_copy(tcptx::smem_u32(&bars[st]), phase, wait_limit_ns, status)) lost[turn] = 1;
+        if (!wait_copy(tcptx::smem_u32(&bars[st]), phase, waits)) buf[turn][16].x = 1.0f;
         const T* in = reinterpret_cast<const T*>(smem + (size_t)(st * arrays) * row_bytes);
         Raw8<T> rw[VPT], rx[VPT], ro[VPT];
         float sq = 0.0f, dot = 0.0f;
@@ -470,12 +464,13 @@ decxb_rmsnorm_backward_rows_kernel(const NormBwdArgs a, const int stages, const 
         }
         /* behind the barrier in here every thread has its values: the stage can be filled again */
         const float2 s = block_sum2(sq, dot, buf[turn], warp, lane, nwarps);
-        if (lost[turn]) {                      /* the row did not come: it and those behind it stay unwritten and out of dgamma */
+        const bool gone = buf[turn][16].x != 0.0f;
+        if (tid == 0 && !gone && row + (int64_t)stages * gridDim.x < a.rows) fetch(row + (int64_t)stages * gridDim.x, st);
+        const float r = rsqrtf(s.x / (float)cols + a.eps), k = r * r * (s.y / (float)cols);
+        if (gone) {                            /* the row did not come: it and those behind it stay unwritten and out of dgamma */
             if (tid == 0) drain_copies(bars, stages, st, phase, row, a.rows);
             break;
         }
-        if (tid == 0 && row + (int64_t)stages * gridDim.x < a.rows) fetch(row + (int64_t)stages * gridDim.x, st);
-        const float r = rsqrtf(s.x / (float)cols + a.eps), k = r * r * (s.y / (float)cols);
 #pragma unroll
         for (int i = 0; i < VPT; ++i) {
             float w[8], x[8], o[8];
@@ -570,8 +565,7 @@ int launch_backward_rows(decxb_ctx* ctx, const NormBwdArgs& a, unsigned grid, in
     static cudaError_t err[DECXB_MAX_DEVICES];
     std::call_once(once[ctx->device], [&] { err[ctx->device] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 225 * 1024); });
     if (err[ctx->device] != cudaSuccess) return decxb_fail(ctx, DECXB_ERR_CUDA, std::string("norm kernel attributes: ") + cudaGetErrorString(err[ctx->device]));
-    return launch_after(ctx, kernel, grid, threads_for(decxb_ceil_div(a.cols, 8), VPT, 512), smem, s, a, stages, ctx->wait_limit_ns, ctx->d_status,
-                        lost_copy(ctx));
+    return launch_after(ctx, kernel, grid, threads_for(decxb_ceil_div(a.cols, 8), VPT, 512), smem, s, a, stages, waits_of(ctx));
 }
 
 template <typename T>

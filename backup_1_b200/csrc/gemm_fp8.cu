@@ -54,9 +54,7 @@ struct Params {
     int d_type;
     bool tma_store;                /* D leaves, and C comes, through the copy engine   */
     bool d_vec;                    /* four results of a row may leave in one store      */
-    int lost_tile;                 /* tile whose last k-block is never brought (tests; -1: none) */
-    long long wait_limit_ns;
-    decxb_dev_status* status;
+    Waits waits;                   /* (of the tile that is `lost` the last k-block is never brought) */
 };
 
 /* True in one lane of a converged warp, always the same one. */
@@ -74,20 +72,17 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const P
     unsigned long long t0 = 0;
     for (uint32_t spins = 1; !__all_sync(0xffffffffu, mbar_try_wait(bar, parity)); ++spins) {
         if ((spins & 1023u) == 0) {
-            bool give_up = false;
+            bool over = false;
             if (elect_one()) {
                 const unsigned long long t = globaltimer_ns();
                 if (t0 == 0) t0 = t;
-                give_up = *reinterpret_cast<volatile int*>(&p.status->code) != 0;
-                if (!give_up && (long long)(t - t0) > p.wait_limit_ns) {
-                    give_up = true;
-                    if (atomicCAS(&p.status->code, 0, DECXB_DEVERR_WAIT_EXPIRED) == 0) {
-                        p.status->where = where; p.status->block = (int)blockIdx.x; p.status->detail = detail;
-                        __threadfence_system();
-                    }
+                over = gave_up(p.waits);
+                if (!over && (long long)(t - t0) > p.waits.limit_ns) {
+                    over = true;
+                    give_up(p.waits, where, detail);
                 }
             }
-            if (__any_sync(0xffffffffu, give_up)) return false;
+            if (__any_sync(0xffffffffu, over)) return false;
         }
     }
     return true;
@@ -422,7 +417,7 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
                         /* both CTAs' bytes are counted on the leader's barrier */
                         if (is_leader) mbar_arrive_expect_tx(full_bar(stage), 2 * C::STAGE_BYTES);
                         const uint32_t fb = mapa(full_bar(stage), 0);
-                        if (t != p.lost_tile || kb + 1 < p.num_kb) {
+                        if (t != (int)p.waits.lost || kb + 1 < p.num_kb) {
                             tma_load_2d_pair(stage_a(stage), &map_a, fb, kb * BK, row_a);
                             tma_load_2d_pair(stage_b(stage), &map_b, fb, kb * BK, row_b);
                         }
@@ -436,7 +431,7 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
             /* a wait gave up somewhere: wait (with a limit) for the copies that are still on their way into
              * shared memory; the leader's barriers count its peer's as well, but for a stage that only the peer had filled
              * again, which the peer gives some time */
-            if (lane == 0 && *reinterpret_cast<volatile int*>(&p.status->code) != 0) {
+            if (lane == 0 && gave_up(p.waits)) {
                 for (int s2 = 0; is_leader && s2 < C::STAGES; ++s2) {
                     if (!((armed >> s2) & 1u)) continue;
                     for (int tries = 0; tries < 2048 && !mbar_try_wait(full_bar(s2), (armed_parity >> s2) & 1u); ++tries)
@@ -729,7 +724,7 @@ decxb_gemm_fp8_split_kernel(const __grid_constant__ CUtensorMap map_w, const __g
 
     if (warp == 0) {
         /* ------------------------------------------------------------ TMA producer ---- */
-        const int lost_kb = tile == p.lost_tile && rank == 0 ? kb_last - 1 : -1;
+        const int lost_kb = tile == (int)p.waits.lost && rank == 0 ? kb_last - 1 : -1;
         int stage = 0; uint32_t phase = 0;
         uint32_t armed = 0, armed_parity = 0;
         for (int kb = kb_first; kb < kb_last; ++kb) {
@@ -747,7 +742,7 @@ decxb_gemm_fp8_split_kernel(const __grid_constant__ CUtensorMap map_w, const __g
             armed_parity = (armed_parity & ~(1u << stage)) | (phase << stage);
             if (++stage == stages) { stage = 0; phase ^= 1u; }
         }
-        if (lane == 0 && *reinterpret_cast<volatile int*>(&p.status->code) != 0) {       /* copies still on their way */
+        if (lane == 0 && gave_up(p.waits)) {       /* copies still on their way */
             for (int s2 = 0; s2 < stages; ++s2) {
                 if (!((armed >> s2) & 1u)) continue;
                 for (int tries = 0; tries < 2048 && !mbar_try_wait(full_bar(s2), (armed_parity >> s2) & 1u); ++tries) __nanosleep(64);
@@ -1129,8 +1124,7 @@ int gemm_fp8(decxb_ctx* ctx, const decxb_fp8_matrix* pa, const decxb_fp8_matrix*
         /* the copy engine clips a store at the array's edge in whole 16-byte pieces, so N has to be made of them too */
         p.tma_store = aligned(D, ldd * e, 16) && (!C || aligned(C, ldc * e, 16)) && N * e % 16 == 0;
         p.d_vec = aligned(D, ldd * e, 4 * e);
-        p.wait_limit_ns = ctx->wait_limit_ns; p.status = ctx->d_status;
-        p.lost_tile = (int)lost_copy(ctx);
+        p.waits = waits_of(ctx);
         rc = launch_product(ctx, A, B, p, s);
     }
     if (a_copy) decxb_free_on_stream(ctx, a_copy, s);

@@ -293,7 +293,13 @@ DECXB_API int decxb_gemm_f32_noalloc(int device, int64_t M, int64_t N, int64_t K
  * These entries leave the calling thread's current device as it was, are asynchronous on `stream`,
  * may run at the same time on several streams, and take no scratch memory unless said so at the
  * entry; calls that take none may be captured into a CUDA graph.  A size of zero rows is a call
- * without work (DECXB_OK).  Overlap of an output with an input is allowed where the entry says so. */
+ * without work (DECXB_OK).  Overlap of an output with an input is allowed where the entry says so.
+ *
+ * A wait inside a kernel that lasts longer than decxb_set_wait_limit_ms gives up: what its block had still to do is left
+ * unwritten (and out of dgamma).  The call has returned DECXB_OK by then; decxb_synchronize returns DECXB_ERR_TIMEOUT.  So a program that
+ * synchronises its own streams can rely on the results once decxb_synchronize, which waits for the whole device, has
+ * returned DECXB_OK after them.  Other calls are not affected; replays of the same captured call may end early until
+ * decxb_synchronize has reported it. */
 typedef enum decxb_dtype { DECXB_F32 = 0, DECXB_F16 = 1, DECXB_BF16 = 2 } decxb_dtype;
 typedef enum decxb_fp8_type {
     DECXB_FP8_E4M3 = 0,      /* largest value 448, no infinity                    */

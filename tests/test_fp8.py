@@ -1311,3 +1311,49 @@ def test_tensor_probes_of_two_contexts_beside_products(ctx):
     assert len(rates) == 2 and min(rates) > 0
     for _, _, D, want in made:
         assert torch.equal(D, want)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["norm", "backward", "few tiles", "many tiles"])
+def test_a_wait_that_gave_up_does_not_cut_later_calls_short(ctx, kind):
+    """Two calls whose copies are lost, nothing asked between: the second waits for its own limit, and a third that loses nothing is whole."""
+    import time
+
+    g = gen(37)
+    if kind in ("norm", "backward"):
+        rows, cols = 8 * 2 * sms(), 2304
+        x, gamma, Y = torch.randn(rows, cols, device=DEV, generator=g).bfloat16(), torch.ones(cols, device=DEV), torch.empty(rows, cols, device=DEV, dtype=torch.bfloat16)
+        if kind == "norm":
+            call = lambda: ctx.rmsnorm(rows, cols, x, cols, gamma, 1e-6, Y=Y, ldy=cols, stream=cur())  # noqa: E731
+        else:
+            call = lambda: ctx.rmsnorm_backward(rows, cols, x, cols, x, cols, gamma, 1e-6, Y, cols, stream=cur())  # noqa: E731
+    else:
+        M, N, K = (4, 512, 2048) if kind == "few tiles" else (2048, 1280, 384)
+        A, _ = int_matrix(g, M, K, b.FP8_E4M3, 1)
+        B, _ = int_matrix(g, N, K, b.FP8_E4M3, 128)
+        Y = torch.empty(M, N, device=DEV)
+        call = lambda: ctx.gemm_fp8(A, B, Y, N, stream=cur())  # noqa: E731
+    call()
+    ctx.synchronize()
+    want = Y.clone()
+    try:
+        ctx.set_wait_limit_ms(400)
+        took = []
+        for _ in range(2):
+            ctx.L.decxb_inject_lost_copy(ctx.h, 0)
+            t0 = time.perf_counter()
+            call()
+            torch.cuda.synchronize()
+            took.append(time.perf_counter() - t0)
+        Y.zero_()
+        call()
+        torch.cuda.synchronize()
+        assert torch.equal(Y, want)
+        with pytest.raises(b.DecxbError) as e:
+            ctx.synchronize()
+        assert e.value.status == 103
+        assert min(took) >= 0.4, took
+    finally:
+        ctx.L.decxb_inject_lost_copy(ctx.h, -1)
+        ctx.set_wait_limit_ms(1000)
+    ctx.synchronize()
