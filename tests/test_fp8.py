@@ -1357,3 +1357,85 @@ def test_a_wait_that_gave_up_does_not_cut_later_calls_short(ctx, kind):
         ctx.L.decxb_inject_lost_copy(ctx.h, -1)
         ctx.set_wait_limit_ms(1000)
     ctx.synchronize()
+
+
+# ---- loops over many rows, and every form of a kernel -------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("dtype,gtype", [(torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32), (torch.float32, torch.float32)])
+@pytest.mark.parametrize("rows,cols", [(10000, 64), (10000, 250), (6001, 1032), (3001, 4096), (1301, 5120), (701, 9008), (1301, 5121), (701, 16400), (2501, 2044)])
+def test_norm_backward_of_more_rows_than_blocks(ctx, rows, cols, dtype, gtype):
+    """Every block (up to 256 columns: every warp) takes several rows: stages that are filled again, sums that alternate, dgamma over the rows of a block;
+    dX apart, in place of dY and in place of dR gives the same bits.  Bounds as in test_norm_backward."""
+    blocks = ctx.rmsnorm_backward_workspace(rows, cols) // (4 * cols)
+    at_once = blocks * (8 if cols <= 256 else 1)
+    assert rows > 2 * at_once or (cols <= 256 and rows > at_once)
+    g = gen(rows + 5 * cols)
+    h, dy, dr = (torch.randn(rows, cols, device=DEV, generator=g).to(dtype) for _ in range(3))
+    gamma = (1 + 0.2 * torch.randn(cols, device=DEV, generator=g)).to(gtype)
+    n = ctx.rmsnorm_backward_workspace(rows, cols)
+    ws = torch.empty(n, device=DEV, dtype=torch.uint8)
+    longest = -(-rows // blocks) + -(-blocks // 32) + 6
+    wide = 1.0 if cols <= 16384 else cols / 16384 * 4
+    small = 2.0 ** -25 if dtype == torch.float16 else 0.0
+
+    def run(y, res, dx):
+        dg = torch.full((cols,), float("nan"), device=DEV)
+        ctx.rmsnorm_backward(rows, cols, y, cols, h, cols, gamma, 1e-5, dx, cols, dg, dR=res, lddr=cols, workspace=ws, workspace_bytes=n, stream=cur())
+        ctx.synchronize()
+        return dx, dg
+    for res in (None, dr):
+        dx, dg = run(dy, res, torch.empty_like(h))
+        wx, wg, mx, mg = backward_ref(dy, h, gamma, 1e-5, res)
+        assert bool(((dx.double() - wx).abs() <= HALF[dtype] * wx.abs() * 1.001 + 200 * wide * U * mx + small).all())
+        assert bool(((dg.double() - wg).abs() <= (96 * wide + longest + 4) * U * mg).all())
+        y = dy.clone()
+        again, dg2 = run(y, res, y)
+        assert torch.equal(again, dx) and torch.equal(dg2, dg)
+    r = dr.clone()
+    again, dg2 = run(dy, r, r)
+    assert torch.equal(again, dx) and torch.equal(dg2, dg)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("rows,cols", [(3, 9001), (2, 10240), (3, 16400), (2, 20003), (2, 32760), (1300, 1028), (40, 5121), (2400, 4096), (5000, 200)])
+def test_norm_of_rows_that_need_several_vectors_a_thread_and_ragged_ones(ctx, rows, cols, dtype):
+    g = gen(rows + cols)
+    x, r = (torch.randn(rows, cols, device=DEV, generator=g).to(dtype) for _ in range(2))
+    gamma = (1 + 0.2 * torch.randn(cols, device=DEV, generator=g)).to(dtype)
+    h, y = norm_ref(x, r, gamma, 1e-5)
+    H, Y, Q = torch.empty_like(x), torch.empty_like(x), b.Fp8Matrix.empty(rows, cols)
+    ctx.rmsnorm(rows, cols, x, cols, gamma, 1e-5, R=r, ldr=cols, H=H, ldh=cols, Y=Y, ldy=cols, Q=Q, stream=cur())
+    ctx.synchronize()
+    assert near(H, h, dtype, U if dtype == torch.float32 else 2 * U) and near(Y, y, dtype, NORM_U)
+    s = want_scales(blocks_amax(y, 1), b.FP8_E4M3, b.SCALE_AMAX).double()
+    assert bool(((Q.scales.double() - s).abs() <= (NORM_U + 2 * U) * s).all())
+    check_codes(Q.data, y / spread(Q.scales, 1, rows, cols).double(), b.FP8_E4M3, NORM_U + 4 * U)
+
+
+@gpu
+@pytest.mark.parametrize("M", [1, 16, 17, 32, 40, 64, 100])
+@pytest.mark.parametrize("N,K", [(1000, 8200), (1024, 1024), (4096, 2048), (4090, 4100), (6000, 4096), (12000, 1000), (20000, 640), (40000, 130)])
+def test_product_of_few_tokens_in_every_cut(ctx, M, N, K):
+    """Eight, four, two shares of K and one, one block to an SM and two, over one wave and several."""
+    g = gen(M + N + K)
+    A, a = int_matrix(g, M, K, b.FP8_E4M3, 1, pad=-K % 16)
+    B, w = int_matrix(g, N, K, b.FP8_E4M3, 128, pad=-K % 16)
+    assert torch.equal(run_gemm(ctx, A, B, torch.float32).double(), a @ w.t())
+
+
+@gpu
+@pytest.mark.parametrize("dims", [(40, 1024, 520), (1500, 2304, 256), (3000, 640, 384)])
+def test_layers_norm_and_its_gradients_within_the_layer(ctx, dims):
+    """What Layer.check leaves out: the sum, the norm's output, dx and dgamma, each on what it was given."""
+    layer = Layer(ctx, *dims)
+    layer.step()
+    ctx.synchronize()
+    bf = torch.bfloat16
+    h, y = norm_ref(layer.x, layer.r, layer.gamma, 1e-6)
+    assert near(layer.h, h, bf, 2 * U) and near(layer.y, y, bf, NORM_U)
+    wx, wg, mx, mg = backward_ref(layer.dy, layer.h, layer.gamma, 1e-6, layer.x)
+    parts = layer.ws.numel() // (4 * dims[1])
+    longest = -(-dims[0] // parts) + -(-parts // 32) + 6
+    assert bool(((layer.dx.double() - wx).abs() <= HALF[bf] * wx.abs() * 1.001 + 200 * U * mx).all())
+    assert bool(((layer.dgamma.double() - wg).abs() <= (96 + longest + 4) * U * mg).all())
