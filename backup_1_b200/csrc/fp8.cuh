@@ -131,8 +131,8 @@ __device__ __forceinline__ float max_nan(float a, float b)
     float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r;
 }
 
-/* amax / largest value, correctly rounded (a product with the reciprocal and one correction by the remainder), then the
- * rule; infinity and NaN pass. */
+/* amax / largest value, correctly rounded (a product with the reciprocal and one correction by the remainder, Markstein's
+ * method), then the rule; infinity and NaN pass. */
 __device__ __forceinline__ float scale_of(float amax, int type, int rule)
 {
     const float most = type == DECXB_FP8_E4M3 ? 448.0f : 57344.0f, inv = type == DECXB_FP8_E4M3 ? 1.0f / 448.0f : 1.0f / 57344.0f;
@@ -148,7 +148,7 @@ __device__ __forceinline__ float scale_of(float amax, int type, int rule)
 
 /* What a block's scale does to its values.  With the amax rule x / s of 16-bit x often lies half way between two codes but for
  * the rounding of s itself, so a product with 1 / s alone, one step of fp32 off, turns four codes in ten thousand
- * over: one correction by the remainder x - q s makes it the fp32 quotient.  (With the power-of-two rule the product is
+ * over: one correction by the remainder x - q s (Markstein's) makes it the fp32 quotient.  (With the power-of-two rule the product is
  * exact and the remainder 0.) */
 struct alignas(8) Quantiser { float inv, minus_s; };    /* 1 / scale, and -scale (0 for an infinite one, whose finite values give 0) */
 __device__ __forceinline__ Quantiser quantiser(float scale)

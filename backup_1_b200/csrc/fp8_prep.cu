@@ -171,8 +171,9 @@ decxb_rmsnorm_kernel(const NormArgs a)
  * `stages` rows ahead, one vector a thread.  Against a block per row (above) there is always something on the way, and
  * what does not depend on the row (gamma, addresses) is done once: the instructions of 16-bit rows bound that
  * kernel (43 an element, 73 % of the issue slots).
- * Two blocks to an SM, each two rows ahead: 51.5 us for 8192 x 4096 with the sum, the plain and the fp8 output (5.9 TB/s); four rows
- * ahead 52.5, three blocks 56, and compiled for the registers of two blocks 64, with the same counts of
+ * Two blocks to an SM, each two rows ahead: 52.1 us for 8192 x 4096 with the sum, the plain and the fp8 output (5.8 TB/s in a graph; called
+ * one after another 54 to 56, singly on an idle device 63). Before the blocks asked whether a row had come it was 51.1, and then
+ * four rows ahead 52.5, three blocks 56, and compiled for the registers of two blocks 64, with the same counts of
  * instructions: reads and writes share the memory best when neither runs far ahead. */
 template <typename T>
 __global__ void __launch_bounds__(512, 3)
@@ -321,7 +322,7 @@ template <typename T>
 int launch_norm(decxb_ctx* ctx, const NormArgs& a, cudaStream_t s)
 {
     const int64_t nvec = decxb_ceil_div(a.cols, 8);
-    /* 16-bit rows of 2049 to 4096 columns, eight or more to an SM: 8192 x 4096 60.6 us with a block a row, 51.5 with rows by bulk
+    /* 16-bit rows of 2049 to 4096 columns, eight or more to an SM: 8192 x 4096 60.6 us with a block a row, 52.1 with rows by bulk
      * copies; but 600 x 4096 5.6 and 7.0, 16384 x 1024 29 and 58, 4096 x 4096 fp32 46.6 and 53.8 */
     if constexpr (sizeof(T) == 2)
         if (a.vec && a.gvec && a.cols % 8 == 0 && (!a.q || a.qvec) && a.cols > 2048 && a.cols <= 4096 && a.rows >= 8 * (int64_t)ctx->sm_count)
@@ -402,7 +403,7 @@ decxb_rmsnorm_backward_kernel(const NormBwdArgs a)
 
 /* A block per row, its rows arriving in shared memory by bulk copies `stages` rows ahead: a row is a chain of load, sum over
  * the block, store, and without the copies a block would have nothing on the way during most of it (8192 x 4096 bf16:
- * 122 us with loads into registers). */
+ * 122 us with loads into registers, 47.8 so, 5.6 TB/s). */
 template <typename T, int VPT>
 __global__ void __launch_bounds__(512, VPT == 1 ? 2 : 1)
 decxb_rmsnorm_backward_rows_kernel(const NormBwdArgs a, const int stages, const Waits waits)

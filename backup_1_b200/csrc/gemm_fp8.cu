@@ -314,7 +314,7 @@ __device__ __forceinline__ void put4(const Params& p, int64_t row, int64_t col, 
 
 /* --------------------------------------------------------------------------------------
  * Many result tiles: a pair of CTAs (cta_group::2) per tile of 256 x 256, each with 128 rows of A and 128 of B.
- * 16384 x 4096 x 8192 takes 480 to 530 us (2.1 to 2.3 PFLOP/s, the SM clock near 1.55 GHz under the power cap). A k-block costs 880
+ * 16384 x 4096 x 8192 takes 440 to 520 us (2.1 to 2.5 PFLOP/s, the SM clock near 1.55 GHz under the power cap). A k-block costs some 890
  * clocks of an SM where the tensor core needs 512: feeding the tiles alone takes 231 us of that size, the MMAs alone
  * about 440, reading tensor memory and adding alone 393, and the last two overlap only in part, two accumulators being
  * all that tensor memory holds. With a factor per column two operations an element, and what the
@@ -648,7 +648,7 @@ decxb_gemm_fp8_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_co
  * k-blocks each, and their fp32 sums meet through distributed shared memory: no workspace, no atomics, one order.
  * Bound by the weights' bytes for few tokens (a k-block brings 16 KiB of B whatever NT is): 1 x 8192 x 8192 4.4 TB/s,
  * 64 x 16384 x 16384 5.7 TB/s; below some 30 MB by a launch's 2.4 us and the length of one pass through the pipeline
- * (1 x 4096 x 4096: 5.6 us).
+ * (1 x 4096 x 4096: 5.3 us).
  * Tensor memory is read in the shape in which a thread holds two adjacent columns of every eight for four rows
  * (16x256b), so that a warp's column factors come in a quarter of the shared-memory reads of one row a thread.
  * ------------------------------------------------------------------------------------ */

@@ -344,7 +344,8 @@ DECXB_API int decxb_quantize_fp8(decxb_ctx* ctx, int x_type, int64_t rows, int64
  *   h = X + R (R may be NULL: h = X),  y = h / sqrt(mean(h^2) + eps) * gamma.
  * Writes what is given of H (h, rounded to `type`), Y (y, rounded to `type`) and Q (y quantised as
  * decxb_quantize_fp8 does, block_rows 1); at least one of the three.  X, R, H, Y are [rows][cols] of
- * `type`, gamma is cols values of gamma_type; statistics, h and y are fp32 until they are rounded.
+ * `type`, gamma is cols values of gamma_type; statistics, h and y are fp32 until they are rounded, so the sum of a row's
+ * squares has to be finite in fp32 (|h| below 1e17 at 32768 columns; an infinite sum makes the row's y zero).
  * H or Y may be X or R itself (same pointer and leading dimension), H and Y are different. */
 DECXB_API int decxb_rmsnorm(decxb_ctx* ctx, int type, int64_t rows, int64_t cols, const void* X, int64_t ldx,
                             const void* R, int64_t ldr, const void* gamma, int gamma_type, float eps,
