@@ -38,9 +38,10 @@ extern "C" const char* decxb_status_string(int status)
 }
 
 /* The calling thread's own last failure, and the context it was on: threads that share a context each read the text of their
- * own call, and no thread's text is written while another reads it. */
+ * own call, and no thread's text is written while another reads it.  Plain arrays: a context may be destroyed when the thread's objects
+ * already are. */
 static thread_local uint64_t own_error_ctx = 0;
-static thread_local std::string own_error, others_error;
+static thread_local char own_error[1024], others_error[1024];
 
 void decxb_set_error(decxb_ctx* ctx, const std::string& msg)
 {
@@ -49,7 +50,7 @@ void decxb_set_error(decxb_ctx* ctx, const std::string& msg)
         std::lock_guard<std::mutex> lock(ctx->error_mtx);
         ctx->last_error = msg;
     }
-    own_error = msg;
+    snprintf(own_error, sizeof own_error, "%s", msg.c_str());
     own_error_ctx = ctx->serial;
 }
 
@@ -62,10 +63,10 @@ int decxb_fail(decxb_ctx* ctx, int status, const std::string& msg)
 extern "C" const char* decxb_last_error(decxb_ctx* ctx)
 {
     if (!ctx) return "null context";
-    if (own_error_ctx == ctx->serial) return own_error.c_str();
+    if (own_error_ctx == ctx->serial) return own_error;
     std::lock_guard<std::mutex> lock(ctx->error_mtx);
-    others_error = ctx->last_error;
-    return others_error.c_str();
+    snprintf(others_error, sizeof others_error, "%s", ctx->last_error.c_str());
+    return others_error;
 }
 
 int decxb_bind(decxb_ctx* ctx)
