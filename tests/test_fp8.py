@@ -1439,3 +1439,20 @@ def test_layers_norm_and_its_gradients_within_the_layer(ctx, dims):
     longest = -(-dims[0] // parts) + -(-parts // 32) + 6
     assert bool(((layer.dx.double() - wx).abs() <= HALF[bf] * wx.abs() * 1.001 + 200 * U * mx).all())
     assert bool(((layer.dgamma.double() - wg).abs() <= (96 + longest + 4) * U * mg).all())
+
+
+@gpu
+@pytest.mark.parametrize("M", [3, 300])
+@pytest.mark.parametrize("rows_apart,blocks_apart", [(0, 0), (1, 0), (0, 1), (7, 3)])
+def test_product_of_scales_shared_by_stride(ctx, M, rows_apart, blocks_apart):
+    """One scale for a whole operand, for all of a row, for all rows of a block column, and scales with gaps."""
+    g = gen(41)
+    N, K = 260, 640
+    made = []
+    for n in (M, N):
+        code = torch.randint(-4, 5, (n, K), device=DEV, generator=g).float().to(torch.float8_e4m3fn)
+        s = torch.exp2(torch.randint(-2, 3, (n * rows_apart + 5 * blocks_apart + 1,), device=DEV, generator=g).float())
+        at = (torch.arange(n, device=DEV)[:, None] * rows_apart + (torch.arange(K, device=DEV) // 128)[None, :] * blocks_apart)
+        made.append((b.Fp8Matrix(code, s, n, K, K, rows_apart, blocks_apart), code.double() * s.double()[at]))
+    (A, a), (B, w) = made
+    assert torch.equal(run_gemm(ctx, A, B, torch.float32).double(), a @ w.t())
