@@ -549,7 +549,9 @@ decxb_column_sum_kernel(const float* part, int parts, int64_t cols, float* out)
 }
 
 /* Blocks to an SM, whose sums are the rows of the workspace: more of them where rows are short and a block's chain of load,
- * sum and store has little to move (16384 x 1024: 2 blocks and a warp a row 101 us). */
+ * sum and store has little to move (16384 x 1024: 2 blocks and a warp a row 101 us).  From 4097 to 8192 columns two are planned and
+ * the kernel's 122 registers let one on at a time; the other's shared memory is what fp32 rows of 4696 columns and more (three arrays; 7048,
+ * two) lack for a second stage, so that those take the kernel that reads rows twice. */
 constexpr int64_t WARP_COLS = 256;
 int64_t backward_per_sm(int64_t cols) { return cols <= WARP_COLS ? 4 : cols <= 1024 ? 8 : cols <= 2048 ? 4 : cols <= 8192 ? 2 : 1; }
 int64_t backward_blocks(const decxb_ctx* ctx, int64_t rows, int64_t cols)
